@@ -266,6 +266,86 @@ int nxt_paged_kv_copy_slots(void *key_cache, void *value_cache, const int *src_s
                             int block_size, int kv_block_stride, int kv_head_stride, int kv_dtype,
                             nxt_stream_t stream);
 
+/* ------------------------------------------------------- 4-bit K/V cache
+ * No counterpart in the reference.  A paged cache that holds K and V in 4
+ * bits a channel with a range per 32 channels: 5/8 of a byte a channel, 3.2
+ * times the tokens of an fp16 cache in the same memory.  Rows are quantised as
+ * they are written and stay as they are; the attention reads the codes.
+ *
+ * Format.  A row (one token, one kv head) is cut into groups of 32 channels
+ * (the last one of head_size 80 and 112 has 16).  Per group, in fp32
+ * arithmetic, with x clamped to +-65504:
+ *   low  = fp16(min x)        step = fp16((max x - min x) * fp32(1 / 15))
+ *   code = rint((x - low) * (1 / step)) clamped to 0..15; 0 where step is 0
+ *   the value stored is low + step * code
+ * so an element is off by half a step at most, plus the rounding of low and
+ * step (fp16, which below 2^-14 is absolute: 2^-25 for low, up to 15 * 2^-25
+ * for step).  A NaN makes low and step NaN: its whole group reads back as NaN.
+ * Infinities are stored as +-65504.
+ * Caches: `key_cache` and `value_cache` are bytes, page b of kv head h at
+ * b*kv_block_stride + h*kv_head_stride (BYTES here, multiples of 16), each
+ * nxt_paged_kv4_page_bytes(head_size, block_size) long; the layout inside a
+ * page is the library's (xllms_amd/csrc/kv4_layout.h), the same for every row
+ * dtype.  block_size: a power of two in [16, 1024].  `dtype` (NxtKvDtype) is
+ * that of the rows, the query and the output, and need not be the same from
+ * call to call on one cache.
+ * All calls are asynchronous on `stream` and return NXT_ATTN_OK or a negative
+ * status (also recorded for nxt_attn_last_status); a refused call launches
+ * nothing.  The caller owns every buffer and guarantees that page ids and
+ * slots lie inside the cache. */
+
+/* Bytes of one page of one kv head (of K, and as many of V), or a negative
+ * status. */
+int nxt_paged_kv4_page_bytes(int head_size, int block_size);
+
+/* nxt_paged_kv_append for a 4-bit cache: token s's rows (row s of key / value,
+ * [num_seqs][num_kv_heads][head_size] in dtype) are quantised into page
+ * block_tables[s][positions[s] / block_size], slot positions[s] % block_size;
+ * the same positions and page ids skip a token.  No two tokens of one call may
+ * have the same slot. */
+int nxt_paged_kv4_append(void *key_cache, void *value_cache, const void *key, const void *value,
+                         const int *block_tables, const int *positions, int num_seqs,
+                         int num_kv_heads, int head_size, int max_num_blocks_per_seq,
+                         int block_size, int kv_block_stride, int kv_head_stride, int dtype,
+                         nxt_stream_t stream);
+
+/* nxt_paged_kv_write_slots for a 4-bit cache: token i's rows are quantised
+ * into flat slot slot_mapping[i]; a negative slot skips it.  The slots of one
+ * call must differ. */
+int nxt_paged_kv4_write_slots(void *key_cache, void *value_cache, const void *key,
+                              const void *value, const int *slot_mapping, int num_tokens,
+                              int num_kv_heads, int head_size, int block_size,
+                              int kv_block_stride, int kv_head_stride, int dtype,
+                              nxt_stream_t stream);
+
+/* The values held in flat slot slot_mapping[i], low + step * code computed in
+ * fp32 and rounded to dtype, into row i of key / value
+ * ([num_tokens][num_kv_heads][head_size]); a negative slot leaves row i as it
+ * was.  A slot may be named more than once. */
+int nxt_paged_kv4_read_slots(void *key, void *value, const void *key_cache,
+                             const void *value_cache, const int *slot_mapping, int num_tokens,
+                             int num_kv_heads, int head_size, int block_size, int kv_block_stride,
+                             int kv_head_stride, int dtype, nxt_stream_t stream);
+
+/* nxt_paged_kv_copy_slots for a 4-bit cache (the copy-on-write lists of
+ * nxt_kv_seq_admit): codes, lows and steps are copied exactly.  No destination
+ * may be named twice or be the source of another pair in the same call. */
+int nxt_paged_kv4_copy_slots(void *key_cache, void *value_cache, const int *src_slots,
+                             const int *dst_slots, int num_tokens, int num_kv_heads,
+                             int head_size, int block_size, int kv_block_stride,
+                             int kv_head_stride, nxt_stream_t stream);
+
+/* nxt_paged_attention_ex over a 4-bit cache: the same computation and contract
+ * points (empty sequences, negative page ids, lengths past the table, slots
+ * past the length) with K_t and V_t the values stored; query and out in dtype.
+ * num_heads / num_kv_heads <= 64. */
+int nxt_paged_attention_kv4(void *out, const void *query, const void *key_cache,
+                            const void *value_cache, const int *block_tables,
+                            const int *seq_lens, int num_seqs, int num_heads, int head_size,
+                            int num_kv_heads, float scale, int max_num_blocks_per_seq,
+                            int block_size, int kv_block_stride, int kv_head_stride, int dtype,
+                            nxt_stream_t stream);
+
 /* ---------------------------------------------------------- activations
  * The MLP activations of the reference's operator API (include/operator_api.h:
  * 118-150, implemented there by operators/activation_kernels.cu:52-239).

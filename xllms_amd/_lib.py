@@ -65,6 +65,12 @@ OPERATOR_SYMBOLS = (
     "nxt_paged_attention_cascade",
     "nxt_paged_prefix_groups",
     "nxt_paged_kv_copy_slots",
+    "nxt_paged_kv4_page_bytes",
+    "nxt_paged_kv4_append",
+    "nxt_paged_kv4_write_slots",
+    "nxt_paged_kv4_read_slots",
+    "nxt_paged_kv4_copy_slots",
+    "nxt_paged_attention_kv4",
     "nxt_silu_and_mul",
     "nxt_mul_and_silu",
     "nxt_gelu_and_mul",
@@ -140,6 +146,19 @@ def backend(trace: bool = False) -> ctypes.CDLL:
         lib.nxt_paged_prefix_groups.restype = c_int
         lib.nxt_paged_kv_copy_slots.argtypes = [c_void_p] * 4 + [c_int] * 7 + [c_void_p]
         lib.nxt_paged_kv_copy_slots.restype = c_int
+        lib.nxt_paged_kv4_page_bytes.argtypes = [c_int] * 2
+        lib.nxt_paged_kv4_page_bytes.restype = c_int
+        lib.nxt_paged_kv4_append.argtypes = [c_void_p] * 6 + [c_int] * 8 + [c_void_p]
+        lib.nxt_paged_kv4_append.restype = c_int
+        lib.nxt_paged_kv4_write_slots.argtypes = [c_void_p] * 5 + [c_int] * 7 + [c_void_p]
+        lib.nxt_paged_kv4_write_slots.restype = c_int
+        lib.nxt_paged_kv4_read_slots.argtypes = [c_void_p] * 5 + [c_int] * 7 + [c_void_p]
+        lib.nxt_paged_kv4_read_slots.restype = c_int
+        lib.nxt_paged_kv4_copy_slots.argtypes = [c_void_p] * 4 + [c_int] * 6 + [c_void_p]
+        lib.nxt_paged_kv4_copy_slots.restype = c_int
+        lib.nxt_paged_attention_kv4.argtypes = ([c_void_p] * 6 + [c_int] * 4 + [c_float] +
+                                                [c_int] * 5 + [c_void_p])
+        lib.nxt_paged_attention_kv4.restype = c_int
         for name in ACTIVATION_ENTRY_POINTS:
             fn = getattr(lib, name)
             fn.argtypes = [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]

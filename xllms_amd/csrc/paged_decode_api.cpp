@@ -15,6 +15,8 @@
 #include <vector>
 
 #include "activation.h"
+#include "kv4_cache.h"
+#include "kv4_layout.h"
 #include "paged_decode_cascade.h"
 #include "paged_decode_launch.h"
 #include "paged_decode_params.h"
@@ -1034,6 +1036,135 @@ int kv_append_run(void *key_cache, void *value_cache, const void *key, const voi
     return ok();
 }
 
+// --------------------------------------------------------- 4-bit K/V cache
+// Checks common to the operators of a 4-bit cache.
+int kv4_check(int num_kv_heads, int head_size, int block_size, int kv_block_stride,
+              int kv_head_stride) {
+    if (num_kv_heads <= 0) return set_status(NXT_ATTN_E_INVALID, "num_kv_heads %d must be > 0", num_kv_heads);
+    if (!supported_head_size(head_size))
+        return set_status(NXT_ATTN_E_UNSUPPORTED,
+                          "head_size %d not in {32,64,80,96,112,128,192,256}", head_size);
+    if (block_size <= 0) return set_status(NXT_ATTN_E_INVALID, "block_size %d", block_size);
+    if (!is_pow2(block_size) || block_size < xhip::kKv4Tile || block_size > 1024)
+        return set_status(NXT_ATTN_E_UNSUPPORTED,
+                          "block_size %d of a 4-bit cache is not a power of two in [%d, 1024]",
+                          block_size, xhip::kKv4Tile);
+    const long long page = (long long)block_size / xhip::kKv4Tile * xhip::kv4_tile_bytes(head_size);
+    if (kv_block_stride < page || (num_kv_heads > 1 && kv_head_stride < page) || kv_head_stride < 0)
+        return set_status(NXT_ATTN_E_INVALID,
+                          "kv strides (%d, %d bytes) overlap the %lld-byte pages of a kv head",
+                          kv_block_stride, kv_head_stride, page);
+    if ((kv_block_stride | kv_head_stride) & 15)
+        return set_status(NXT_ATTN_E_UNSUPPORTED, "kv strides must be multiples of 16 bytes");
+    return NXT_ATTN_OK;
+}
+
+// Rows into, out of or inside a 4-bit cache: token i's slot from `slots`, or
+// from block_tables + positions.
+int kv4_rows_run(int op, void *key_cache, void *value_cache, void *key, void *value,
+                 const int *slots, const int *src_slots, const int *block_tables,
+                 const int *positions, int num_tokens, int num_kv_heads, int head_size,
+                 int max_num_blocks_per_seq, int block_size, int kv_block_stride,
+                 int kv_head_stride, int dtype, nxt_stream_t stream) {
+    if (dtype != NXT_KV_FP16 && dtype != NXT_KV_BF16 && dtype != NXT_KV_FP32)
+        return set_status(NXT_ATTN_E_UNSUPPORTED, "dtype %d is not FP16/BF16/FP32", dtype);
+    if (num_tokens < 0) return set_status(NXT_ATTN_E_INVALID, "%d tokens < 0", num_tokens);
+    const bool by_table = block_tables || positions;
+    if (by_table && max_num_blocks_per_seq <= 0)
+        return set_status(NXT_ATTN_E_INVALID, "max_num_blocks_per_seq %d must be > 0",
+                          max_num_blocks_per_seq);
+    const int st = kv4_check(num_kv_heads, head_size, block_size, kv_block_stride, kv_head_stride);
+    if (st != NXT_ATTN_OK) return st;
+    const long long max_ctx = by_table ? (long long)max_num_blocks_per_seq * block_size : 0;
+    if (max_ctx > (1LL << 28))
+        return set_status(NXT_ATTN_E_UNSUPPORTED, "context bound %lld tokens too large", max_ctx);
+    if (num_kv_heads > (1 << 24))
+        return set_status(NXT_ATTN_E_UNSUPPORTED, "num_kv_heads %d too large", num_kv_heads);
+    if (num_tokens == 0) return ok();
+    const bool copy = op == xhip::KV4_COPY;
+    if (!key_cache || !value_cache || (!copy && (!key || !value)) || (copy && !src_slots) ||
+        (by_table ? !block_tables || !positions : !slots))
+        return set_status(NXT_ATTN_E_INVALID, "NULL pointer");
+    if (((uintptr_t)key_cache | (uintptr_t)value_cache | (uintptr_t)key | (uintptr_t)value) & 15)
+        return set_status(NXT_ATTN_E_UNSUPPORTED, "tensors must be 16-byte aligned");
+    if (((uintptr_t)slots | (uintptr_t)src_slots | (uintptr_t)block_tables | (uintptr_t)positions) & 3)
+        return set_status(NXT_ATTN_E_INVALID, "int32 arrays must be 4-byte aligned");
+    xhip::Kv4RowParams p;
+    memset(&p, 0, sizeof(p));
+    p.key_cache = (char *)key_cache;
+    p.value_cache = (char *)value_cache;
+    p.key = key;
+    p.value = value;
+    p.slots = by_table ? nullptr : slots;
+    p.src_slots = src_slots;
+    p.block_tables = block_tables;
+    p.positions = positions;
+    p.kv_block_stride = kv_block_stride;
+    p.kv_head_stride = kv_head_stride;
+    p.num_tokens = num_tokens;
+    p.num_kv_heads = num_kv_heads;
+    p.head_size = head_size;
+    p.block_size = block_size;
+    p.bs_shift = ilog2(block_size);
+    p.max_blocks = max_num_blocks_per_seq;
+    p.max_ctx = (int)max_ctx;
+    const hipError_t e = xhip::launch_kv4_rows(p, op, dtype, (hipStream_t)stream);
+    if (e != hipSuccess)
+        return set_status(NXT_ATTN_E_HIP, "4-bit cache rows launch: %s", hipGetErrorString(e));
+    return ok();
+}
+
+int kv4_attention_run(void *out, const void *query, const void *key_cache, const void *value_cache,
+                      const int *block_tables, const int *seq_lens, int num_seqs, int num_heads,
+                      int head_size, int num_kv_heads, float scale, int max_num_blocks_per_seq,
+                      int block_size, int kv_block_stride, int kv_head_stride, int dtype,
+                      nxt_stream_t stream_handle) {
+    if (dtype != NXT_KV_FP16 && dtype != NXT_KV_BF16 && dtype != NXT_KV_FP32)
+        return set_status(NXT_ATTN_E_UNSUPPORTED, "dtype %d is not FP16/BF16/FP32", dtype);
+    if (num_seqs < 0) return set_status(NXT_ATTN_E_INVALID, "num_seqs %d < 0", num_seqs);
+    if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads)
+        return set_status(NXT_ATTN_E_INVALID,
+                          "num_heads %d must be a positive multiple of num_kv_heads %d", num_heads,
+                          num_kv_heads);
+    const int group = num_heads / num_kv_heads;
+    if (group > xhip::kMfmaMaxGroup)
+        return set_status(NXT_ATTN_E_UNSUPPORTED, "GQA group %d > %d", group, xhip::kMfmaMaxGroup);
+    if (max_num_blocks_per_seq <= 0)
+        return set_status(NXT_ATTN_E_INVALID, "max_num_blocks_per_seq %d must be > 0",
+                          max_num_blocks_per_seq);
+    if (!isfinite(scale)) return set_status(NXT_ATTN_E_INVALID, "scale is not finite");
+    const int st = kv4_check(num_kv_heads, head_size, block_size, kv_block_stride, kv_head_stride);
+    if (st != NXT_ATTN_OK) return st;
+    const long long max_ctx = (long long)max_num_blocks_per_seq * block_size;
+    if (max_ctx > (1LL << 28))
+        return set_status(NXT_ATTN_E_UNSUPPORTED, "context bound %lld tokens too large", max_ctx);
+    if (num_seqs == 0) return ok();
+    if (!out || !query || !key_cache || !value_cache || !block_tables || !seq_lens)
+        return set_status(NXT_ATTN_E_INVALID, "NULL tensor pointer");
+    if (((uintptr_t)out | (uintptr_t)query | (uintptr_t)key_cache | (uintptr_t)value_cache) & 15)
+        return set_status(NXT_ATTN_E_UNSUPPORTED, "tensors must be 16-byte aligned");
+    if ((uintptr_t)block_tables & 3 || (uintptr_t)seq_lens & 3)
+        return set_status(NXT_ATTN_E_INVALID, "int32 tables must be 4-byte aligned");
+    hipStream_t stream = (hipStream_t)stream_handle;
+    const size_t row = (size_t)num_heads * head_size * elem_bytes(dtype);
+    for (int s0 = 0; s0 < num_seqs; s0 += xhip::kMaxSeqsPerLaunch) {
+        const int nseq = num_seqs - s0 < xhip::kMaxSeqsPerLaunch ? num_seqs - s0 : xhip::kMaxSeqsPerLaunch;
+        DecodeParams p;
+        memset(&p, 0, sizeof(p));
+        p.out = (char *)out + (size_t)s0 * row;
+        fill_batch(p, (const char *)query + (size_t)s0 * row, key_cache, value_cache,
+                   block_tables + (size_t)s0 * max_num_blocks_per_seq, seq_lens + s0, nseq,
+                   num_heads, num_kv_heads, 1, max_num_blocks_per_seq, block_size, kv_block_stride,
+                   kv_head_stride, scale);
+        const hipError_t e = dtype == NXT_KV_FP16   ? xhip::launch_kv4_f16(p, head_size, stream)
+                             : dtype == NXT_KV_BF16 ? xhip::launch_kv4_bf16(p, head_size, stream)
+                                                    : xhip::launch_kv4_f32(p, head_size, stream);
+        if (e != hipSuccess)
+            return set_status(NXT_ATTN_E_HIP, "4-bit decode launch: %s", hipGetErrorString(e));
+    }
+    return ok();
+}
+
 int dtype_from_size(int dtype_size) {
     if (dtype_size == 2) return NXT_KV_FP16;
     if (dtype_size == 4) return NXT_KV_FP32;
@@ -1260,6 +1391,63 @@ __attribute__((visibility("default"))) int nxt_paged_kv_copy_slots(
     return kv_append_run(key_cache, value_cache, key_cache, value_cache, dst_slots, nullptr,
                          nullptr, num_tokens, num_kv_heads, head_size, 0, block_size,
                          kv_block_stride, kv_head_stride, kv_dtype, stream, src_slots);
+}
+
+__attribute__((visibility("default"))) int nxt_paged_kv4_page_bytes(int head_size, int block_size) {
+    const int st = kv4_check(1, head_size, block_size, 0x7FFFFFF0, 0);
+    if (st != NXT_ATTN_OK) return st;
+    (void)ok();
+    return block_size / xhip::kKv4Tile * xhip::kv4_tile_bytes(head_size);
+}
+
+__attribute__((visibility("default"))) int nxt_paged_kv4_append(
+    void *key_cache, void *value_cache, const void *key, const void *value,
+    const int *block_tables, const int *positions, int num_seqs, int num_kv_heads, int head_size,
+    int max_num_blocks_per_seq, int block_size, int kv_block_stride, int kv_head_stride, int dtype,
+    nxt_stream_t stream) {
+    if ((!block_tables || !positions) && num_seqs > 0)
+        return set_status(NXT_ATTN_E_INVALID, "NULL block_tables / positions");
+    return kv4_rows_run(xhip::KV4_WRITE, key_cache, value_cache, (void *)key, (void *)value, nullptr,
+                        nullptr, block_tables, positions, num_seqs, num_kv_heads, head_size,
+                        max_num_blocks_per_seq, block_size, kv_block_stride, kv_head_stride, dtype,
+                        stream);
+}
+
+__attribute__((visibility("default"))) int nxt_paged_kv4_write_slots(
+    void *key_cache, void *value_cache, const void *key, const void *value,
+    const int *slot_mapping, int num_tokens, int num_kv_heads, int head_size, int block_size,
+    int kv_block_stride, int kv_head_stride, int dtype, nxt_stream_t stream) {
+    return kv4_rows_run(xhip::KV4_WRITE, key_cache, value_cache, (void *)key, (void *)value,
+                        slot_mapping, nullptr, nullptr, nullptr, num_tokens, num_kv_heads,
+                        head_size, 0, block_size, kv_block_stride, kv_head_stride, dtype, stream);
+}
+
+__attribute__((visibility("default"))) int nxt_paged_kv4_read_slots(
+    void *key, void *value, const void *key_cache, const void *value_cache,
+    const int *slot_mapping, int num_tokens, int num_kv_heads, int head_size, int block_size,
+    int kv_block_stride, int kv_head_stride, int dtype, nxt_stream_t stream) {
+    return kv4_rows_run(xhip::KV4_READ, (void *)key_cache, (void *)value_cache, key, value,
+                        slot_mapping, nullptr, nullptr, nullptr, num_tokens, num_kv_heads,
+                        head_size, 0, block_size, kv_block_stride, kv_head_stride, dtype, stream);
+}
+
+__attribute__((visibility("default"))) int nxt_paged_kv4_copy_slots(
+    void *key_cache, void *value_cache, const int *src_slots, const int *dst_slots, int num_tokens,
+    int num_kv_heads, int head_size, int block_size, int kv_block_stride, int kv_head_stride,
+    nxt_stream_t stream) {
+    return kv4_rows_run(xhip::KV4_COPY, key_cache, value_cache, nullptr, nullptr, dst_slots,
+                        src_slots, nullptr, nullptr, num_tokens, num_kv_heads, head_size, 0,
+                        block_size, kv_block_stride, kv_head_stride, NXT_KV_FP16, stream);
+}
+
+__attribute__((visibility("default"))) int nxt_paged_attention_kv4(
+    void *out, const void *query, const void *key_cache, const void *value_cache,
+    const int *block_tables, const int *seq_lens, int num_seqs, int num_heads, int head_size,
+    int num_kv_heads, float scale, int max_num_blocks_per_seq, int block_size, int kv_block_stride,
+    int kv_head_stride, int dtype, nxt_stream_t stream) {
+    return kv4_attention_run(out, query, key_cache, value_cache, block_tables, seq_lens, num_seqs,
+                             num_heads, head_size, num_kv_heads, scale, max_num_blocks_per_seq,
+                             block_size, kv_block_stride, kv_head_stride, dtype, stream);
 }
 
 #define XLLM_ACTIVATION_ENTRY(name, op)                                                            \

@@ -30,4 +30,10 @@ hipError_t launch_decode_bf16(const DecodeParams &p, int head_size, int head_til
 hipError_t launch_decode_f32(const DecodeParams &p, int head_size, int head_tile, bool mfma,
                              hipStream_t stream, hipEvent_t ev_start, hipEvent_t ev_stop);
 
+// The decode attention over a 4-bit K/V cache (paged_decode_kv4.h), by the
+// dtype of query and output.
+hipError_t launch_kv4_f16(const DecodeParams &p, int head_size, hipStream_t stream);
+hipError_t launch_kv4_bf16(const DecodeParams &p, int head_size, hipStream_t stream);
+hipError_t launch_kv4_f32(const DecodeParams &p, int head_size, hipStream_t stream);
+
 }  // namespace xhip
