@@ -16,7 +16,8 @@
 //        r and group g holds channels 32g + 2r (low nibbles) and 32g + 2r + 1
 //        (high nibbles) of tokens 4a..4a+3, token 4a + j in byte kv4_v_byte(j).
 //   [8 dp, 9 dp)   steps, fp16 [4 token quads][ng][4 tokens]
-//   [9 dp, 10 dp)  lows, fp16.  K: [16 tokens][ng].  V: as the steps.
+//   [9 dp, 10 dp)  lows, fp16.  K: [16 tokens][ng] (ng 3: [16][2], then [16], so
+//                  that no token's words straddle).  V: as the steps.
 // That is the order in which the attention's matrix instructions take their
 // operands: a lane's codes of a tile are ng consecutive words of K (its token,
 // its 8 of each group's 32 channels) and of V (its 4 tokens, its 2 channels of
@@ -47,7 +48,8 @@ constexpr int kv4_step(int ng, int token, int group) {
     return 256 * ng + (((token >> 2) * ng + group) * 4 + (token & 3)) * 2;
 }
 constexpr int kv4_k_low(int ng, int token, int group) {
-    return 288 * ng + (token * ng + group) * 2;
+    return 288 * ng + (ng != 3 ? (token * ng + group) * 2
+                               : group < 2 ? (token * 2 + group) * 2 : 64 + token * 2);
 }
 constexpr int kv4_v_low(int ng, int token, int group) {
     return 288 * ng + (((token >> 2) * ng + group) * 4 + (token & 3)) * 2;

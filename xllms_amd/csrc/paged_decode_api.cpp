@@ -484,6 +484,19 @@ void fill_batch(DecodeParams &p, const void *query, const void *key_cache, const
     p.scale_log2 = scale * 1.4426950408889634f;
 }
 
+// One merge workgroup per segment once the segments alone fill two
+// workgroups per CU, or once the (segment, column chunk) grid would
+// launch more than four workgroups per CU (each costs ~2 ns of
+// dispatch; 32-head tiles have 32 chunks per segment at head_size
+// 128).  Fewer, longer segments of few heads (few sequences, long
+// contexts) take the chunk grid, whose 8 threads per column split
+// the many partials.
+int merge_per_segment(int group, int head_tile, int head_size, int nseq, int segs, int cus) {
+    const int mheads = group < head_tile ? group : head_tile;
+    const long long chunks = (mheads * (head_size / 4) + xhip::kMergeCols - 1) / xhip::kMergeCols;
+    return (long long)nseq * segs >= 2LL * cus || (long long)nseq * segs * chunks > 4LL * cus ? 1 : 0;
+}
+
 int run(void *out, const void *query, const void *key_cache, const void *value_cache,
         const int *block_tables, const int *seq_lens, int num_seqs, int num_heads, int head_size,
         int num_kv_heads, float scale, int max_num_blocks_per_seq, int block_size, int dtype_size,
@@ -699,18 +712,8 @@ int run(void *out, const void *query, const void *key_cache, const void *value_c
         // the partition kernel combines cut segments inside its workgroups
         // (same predicate as the kernel instantiation's)
         p.wg_fix = mfma && xhip::mfma_wg_fixup(tiling.head_tile, head_size) != 0 ? 1 : 0;
-        // One merge workgroup per segment once the segments alone fill two
-        // workgroups per CU, or once the (segment, column chunk) grid would
-        // launch more than four workgroups per CU (each costs ~2 ns of
-        // dispatch; 32-head tiles have 32 chunks per segment at head_size
-        // 128).  Fewer, longer segments of few heads (few sequences, long
-        // contexts) take the chunk grid, whose 8 threads per column split
-        // the many partials.
-        const int mheads = group < tiling.head_tile ? group : tiling.head_tile;
-        const long long chunks = (mheads * (head_size / 4) + xhip::kMergeCols - 1) / xhip::kMergeCols;
         p.merge_per_segment =
-            ((long long)nseq * segs >= 2LL * cus || (long long)nseq * segs * chunks > 4LL * cus) ? 1
-                                                                                                : 0;
+            merge_per_segment(group, tiling.head_tile, head_size, nseq, segs, cus);
         if (nt) {  // the fold lives in the chunk-grid merge
             p.merge_per_segment = 0;
             p.nt_fold = 1;
@@ -1114,6 +1117,12 @@ int kv4_rows_run(int op, void *key_cache, void *value_cache, void *key, void *va
     return ok();
 }
 
+// Plan of the 4-bit decode: tokens of a tile (kKv4TileTokens of the kernel),
+// the smallest range of a wavefront, and the tiles a segment's start costs.
+constexpr int kKv4PlanTile = 32;
+constexpr int kKv4MinTiles = 1;
+constexpr int kKv4SegmentCost = 1;
+
 int kv4_attention_run(void *out, const void *query, const void *key_cache, const void *value_cache,
                       const int *block_tables, const int *seq_lens, int num_seqs, int num_heads,
                       int head_size, int num_kv_heads, float scale, int max_num_blocks_per_seq,
@@ -1145,20 +1154,67 @@ int kv4_attention_run(void *out, const void *query, const void *key_cache, const
         return set_status(NXT_ATTN_E_UNSUPPORTED, "tensors must be 16-byte aligned");
     if ((uintptr_t)block_tables & 3 || (uintptr_t)seq_lens & 3)
         return set_status(NXT_ATTN_E_INVALID, "int32 tables must be 4-byte aligned");
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
+    if (e != hipSuccess) return set_status(NXT_ATTN_E_HIP, "hipGetDevice: %s", hipGetErrorString(e));
     hipStream_t stream = (hipStream_t)stream_handle;
+    const int cus = cu_count(device);
+    // groups of 17 heads and more: two row blocks of 16 on each unpacked tile
+    // (head sizes whose state fits the registers twice)
+    const bool wide = group > xhip::kMfmaHeads && head_size <= xhip::kMfmaWideMaxHeadSize;
+    const int head_tile = wide ? 2 * xhip::kMfmaHeads : xhip::kMfmaHeads;
+    const int head_tiles = (group + head_tile - 1) / head_tile;
+    const int segs = num_kv_heads * head_tiles;
+    const long long seq_units =
+        (long long)segs * ((max_ctx + kKv4PlanTile - 1) / kKv4PlanTile + kKv4SegmentCost);
+    if (seq_units >= kMaxLaunchTiles)
+        return set_status(NXT_ATTN_E_UNSUPPORTED,
+                          "one sequence bounds %lld tiles (kv heads x context); limit %lld", seq_units,
+                          kMaxLaunchTiles);
+    const long long fit = kMaxLaunchTiles / seq_units;
+    const int per_launch = fit < xhip::kMaxSeqsPerLaunch ? (int)fit : xhip::kMaxSeqsPerLaunch;
     const size_t row = (size_t)num_heads * head_size * elem_bytes(dtype);
-    for (int s0 = 0; s0 < num_seqs; s0 += xhip::kMaxSeqsPerLaunch) {
-        const int nseq = num_seqs - s0 < xhip::kMaxSeqsPerLaunch ? num_seqs - s0 : xhip::kMaxSeqsPerLaunch;
+    for (int s0 = 0; s0 < num_seqs; s0 += per_launch) {
+        const int nseq = num_seqs - s0 < per_launch ? num_seqs - s0 : per_launch;
+        const size_t lds = (size_t)(nseq + 1) * sizeof(int);
+        const int occ = dtype == NXT_KV_FP16   ? xhip::kv4_occupancy_f16(head_size, head_tile, lds)
+                        : dtype == NXT_KV_BF16 ? xhip::kv4_occupancy_bf16(head_size, head_tile, lds)
+                                               : xhip::kv4_occupancy_f32(head_size, head_tile, lds);
+        if (occ <= 0)
+            return set_status(NXT_ATTN_E_HIP, "no occupancy for head_size %d %s", head_size,
+                              dtype_name(dtype));
+        // one resident round of wavefronts, but no more than the batch's bound
+        // can keep busy
+        constexpr int wpg = xhip::kMfmaWavesPerGroup;
+        long long waves = (long long)cus * occ * wpg;
+        const long long need = ((long long)nseq * seq_units + kKv4MinTiles - 1) / kKv4MinTiles;
+        if (need < waves) waves = need;
+        waves = (waves + wpg - 1) / wpg * wpg;
+        const size_t o_bytes = align256((size_t)2 * waves * head_tile * head_size * sizeof(float));
+        const size_t ml_bytes = align256((size_t)2 * waves * head_tile * 2 * sizeof(float));
+        WsCache::Lease lease;  // held until this chunk's launches are enqueued
+        const int ws_st = get_workspace(device, stream, o_bytes + ml_bytes + lds + sizeof(int), &lease);
+        if (ws_st != NXT_ATTN_OK) return ws_st;
+        char *ws = (char *)lease.ptr();
         DecodeParams p;
         memset(&p, 0, sizeof(p));
         p.out = (char *)out + (size_t)s0 * row;
         fill_batch(p, (const char *)query + (size_t)s0 * row, key_cache, value_cache,
                    block_tables + (size_t)s0 * max_num_blocks_per_seq, seq_lens + s0, nseq,
-                   num_heads, num_kv_heads, 1, max_num_blocks_per_seq, block_size, kv_block_stride,
-                   kv_head_stride, scale);
-        const hipError_t e = dtype == NXT_KV_FP16   ? xhip::launch_kv4_f16(p, head_size, stream)
-                             : dtype == NXT_KV_BF16 ? xhip::launch_kv4_bf16(p, head_size, stream)
-                                                    : xhip::launch_kv4_f32(p, head_size, stream);
+                   num_heads, num_kv_heads, head_tiles, max_num_blocks_per_seq, block_size,
+                   kv_block_stride, kv_head_stride, scale);
+        p.ws_o = (float *)ws;
+        p.ws_ml = (float *)(ws + o_bytes);
+        p.ws_prefix = (int *)(ws + o_bytes + ml_bytes);
+        p.num_waves = (int)waves;
+        p.min_tiles_per_wave = kKv4MinTiles;
+        p.seg_cost = kKv4SegmentCost;
+        p.segment_split = 1;
+        p.merge_per_segment = merge_per_segment(group, head_tile, head_size, nseq, segs, cus);
+        const auto launch = dtype == NXT_KV_FP16   ? xhip::launch_kv4_f16
+                            : dtype == NXT_KV_BF16 ? xhip::launch_kv4_bf16
+                                                   : xhip::launch_kv4_f32;
+        e = launch(p, head_size, head_tile, stream, t_trace_start, t_trace_partition);
         if (e != hipSuccess)
             return set_status(NXT_ATTN_E_HIP, "4-bit decode launch: %s", hipGetErrorString(e));
     }
