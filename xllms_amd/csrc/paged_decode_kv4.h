@@ -29,17 +29,28 @@
 //     pair j, 4 tokens of a and 4 of b; the even channel from the low nibbles,
 //     the odd one, 16 times as large, from the high ones).  Row i of a block is
 //     channel 32g + 2i (+ 1), so a lane ends with 8 neighbouring channels of
-//     each group.  The second sum is one more MFMA, A = lows (lane: group j).
-//     Weights are scaled by 2^13, which
-//     keeps p * step clear of fp16's subnormals: at 2^13 a step of up to 2
-//     (values that span 30) leaves p * step below 2^14.  A tile with a larger
-//     step is summed on its own with p * step / 2^12 and added back times 2^12.
-//     p * step and p go in as two fp16 parts, hi + lo (22 bits); for a bf16
-//     output, whose half step is 2^-8, as one (half step 2^-11).
+//     each group.  The second sum is one more MFMA, A = lows (lane: group j), of
+//     which row NG is ones: the sum of the weights as they went in.
+//     Weights are scaled by 2^13, which keeps p * step clear of fp16's
+//     subnormals: at 2^13 a step of up to 2 (values that span 30) leaves
+//     p * step below 2^14.  Once a piece meets a larger step its weights are
+//     scaled by 2 instead (steps end at 8734).
+//     p and p * step go in as two fp16 parts, hi + lo (~22 bits), by packed
+//     arithmetic: c = fp16(p_hi step), lo = fp16(p_lo step + (p_hi step - c)),
+//     the difference exact in one fma; for a bf16 output, whose half step is
+//     2^-8, as one (p and p * step rounded once each, 2^-11).
 //
-// Per 32 tokens of a kv head at head_size 128 that is 5120 bytes, and about 230
-// vector instructions and 28-52 MFMAs: the unpacking is 5 instructions per 8
-// codes.
+// Memory.  Each wavefront has two slots of LDS with a raw copy of a tile's four
+// cache tiles (10 dp bytes each), which buffer loads to LDS fill two tiles
+// ahead: the keys' half of a slot is refilled when the scores are done, the
+// values' half after PV.  So each cache byte crosses the vector memory path
+// once (a register load of the steps would read them 16 times), and a whole
+// tile per wavefront stays in flight without registers.  The loads are inline
+// assembly without register outputs, and the waits count them: the compiler's
+// own waits for LDS loads in flight would drain them all.
+//
+// Per 32 tokens of a kv head at head_size 128 that is 5120 bytes, about 210
+// vector instructions (fp16; bf16 165) and 28-52 MFMAs.
 #pragma once
 
 #include "kv4_layout.h"
@@ -54,82 +65,41 @@ constexpr int kKv4Waves = kMfmaWavesPerGroup;
 template <int D> struct Kv4Geometry {
     static constexpr int NG = kv4_groups(D);
     static constexpr int kBytes = kv4_tile_bytes(D);
-    static constexpr int kLowWords = (NG + 1) / 2;  // a token's lows of K
+    static constexpr int kPieces = kBytes / 16;             // 16-byte pieces of a cache tile
+    static constexpr int kFetches = (kPieces + 63) / 64;    // loads of a cache tile
+    static constexpr int kLowWords = (NG + 1) / 2;          // a token's lows of K
+    static constexpr int kSlot = 4 * kBytes;                // K a, K b, V a, V b
+    static constexpr int kHalfFetches = 2 * kFetches;       // loads of K (or V) of a tile
 };
 
-// One lane's share of a cache tile.
-template <int D> struct Kv4Keys {
-    uint32_t code[Kv4Geometry<D>::NG];      // token j, quarter q of each group
-    u32x2 step[Kv4Geometry<D>::NG];         // tokens 4q..4q+3
-    uint32_t low[Kv4Geometry<D>::kLowWords];  // token j
-};
-template <int D> struct Kv4Values {
-    uint32_t code[Kv4Geometry<D>::NG];  // tokens 4q..4q+3, channel pair j of each group
-    u32x2 step[Kv4Geometry<D>::NG];     // tokens 4q..4q+3
-    u32x2 low;                          // tokens 4q..4q+3 of group j (past the groups: the last)
-};
-
-template <int N>
-__device__ __forceinline__ void buf_words(__amdgpu_buffer_rsrc_t r, int off, uint32_t (&w)[N]) {
-    if constexpr (N >= 4) {
-        const u32x4 x = buf_load<4, kStreamPolicy>(r, (uint32_t)off);
+// Starts a cache tile's way to LDS address `lds`: nothing waits for it here.
+// With ok false it touches no memory, and what LDS then holds is not used.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+template <int D>
+__device__ __forceinline__ void kv4_fetch(const char *tile, bool ok, uint32_t lds, int lane) {
+    using G = Kv4Geometry<D>;
+    const uint64_t at = (uint64_t)tile;
+    // (uniform already; said once more where the assembly needs it)
+    const u32x4 rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
+                        (uint32_t)__builtin_amdgcn_readfirstlane((int)((at >> 32) & 0xFFFFu)),
+                        (uint32_t)__builtin_amdgcn_readfirstlane(ok ? G::kBytes : 0), 0x00020000u};
+    lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
+    const uint32_t off = (uint32_t)lane * 16;
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = lane_word(x, i);
-        if constexpr (N > 4) {
-            uint32_t rest[N - 4];
-            buf_words<N - 4>(r, off + 16, rest);
-#pragma unroll
-            for (int i = 4; i < N; i++) w[i] = rest[i - 4];
-        }
-    } else {
-        const u32x4 x = buf_load<N, kStreamPolicy>(r, (uint32_t)off);
-#pragma unroll
-        for (int i = 0; i < N; i++) w[i] = lane_word(x, i);
+    for (int c = 0; c < G::kFetches; c++) {
+        if (64 * c + 64 <= G::kPieces || lane < G::kPieces - 64 * c)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen offset:%3 nt lds"
+                         :
+                         : "s"(lds), "v"(off), "s"(rsrc), "n"(1024 * c)
+                         : "memory", "m0");
     }
 }
+#pragma clang diagnostic pop
 
-template <int NG>
-__device__ __forceinline__ void buf_pairs(__amdgpu_buffer_rsrc_t r, int off, u32x2 (&v)[NG]) {
-    uint32_t w[2 * NG];
-    buf_words<2 * NG>(r, off, w);
-#pragma unroll
-    for (int g = 0; g < NG; g++) v[g] = u32x2{w[2 * g], w[2 * g + 1]};
-}
-
-// Buffer over one cache tile; with ok false every load from it is zero and
-// touches no memory.
-template <int D> __device__ __forceinline__ __amdgpu_buffer_rsrc_t kv4_rsrc(const char *tile, bool ok) {
-    return __builtin_amdgcn_make_buffer_rsrc((void *)tile, (short)0,
-                                             ok ? Kv4Geometry<D>::kBytes : 0, 0x00020000);
-}
-
-template <int D>
-__device__ __forceinline__ void kv4_load_keys(__amdgpu_buffer_rsrc_t r, int lane, Kv4Keys<D> &k) {
-    constexpr int NG = Kv4Geometry<D>::NG;
-    const int j = lane & 15, q = lane >> 4;
-    buf_words<NG>(r, kv4_k_word(NG, j, q, 0), k.code);
-    buf_pairs<NG>(r, kv4_step(NG, 4 * q, 0), k.step);
-    if constexpr (NG == 1) {
-        k.low[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, kv4_k_low(NG, j, 0), 0, kStreamPolicy);
-    } else if constexpr (NG == 3) {
-        uint32_t w[1];
-        buf_words<1>(r, kv4_k_low(NG, j, 0), w);
-        k.low[0] = w[0];
-        k.low[1] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, kv4_k_low(NG, j, 2), 0, kStreamPolicy);
-    } else {
-        buf_words<NG / 2>(r, kv4_k_low(NG, j, 0), k.low);
-    }
-}
-
-template <int D>
-__device__ __forceinline__ void kv4_load_values(__amdgpu_buffer_rsrc_t r, int lane, Kv4Values<D> &v) {
-    constexpr int NG = Kv4Geometry<D>::NG;
-    const int j = lane & 15, q = lane >> 4;
-    buf_words<NG>(r, kv4_v_word(NG, q, j, 0), v.code);
-    buf_pairs<NG>(r, kv4_step(NG, 4 * q, 0), v.step);
-    uint32_t w[2];
-    buf_words<2>(r, kv4_v_low(NG, 4 * q, j < NG ? j : NG - 1), w);
-    v.low = u32x2{w[0], w[1]};
+// Waits until at most N loads that were issued later are in flight.
+template <int N> __device__ __forceinline__ void kv4_wait() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
 
 __device__ __forceinline__ f32x4 mfma_h(u32x4 a, u32x4 b, f32x4 c) {
@@ -236,114 +206,170 @@ __device__ __forceinline__ void kv4_load_query(const DecodeParams &p, const Mfma
 // Running state of one head block: lane (q, j) owns head j.
 template <int D> struct Kv4State {
     f32x4 o[Kv4Geometry<D>::NG][2];  // [group][odd channel], rows 4q..4q+3: 2^-24 and 2^-20 of it
-    f32x4 low;                       // row 4q + i: group 4q + i's sum of p * low
-    float l;                         // this lane's part of the running sum
+    f32x4 low;                       // row 4q + i: group 4q + i's sum of p * low; row NG: the
+                                     // sum of p
     float base;                      // weights of head j are 2^(score - base)
-    float limit;                     // score - base up to which they are kept: 13; -inf
+    float limit;                     // score - base up to which they are kept: `top`; -inf
                                      // (and base 0) before the head's first score
 };
 
-constexpr float kKv4Top = 13.0f;  // log2 of the largest weight
+// log2 of the largest weight, before and after a piece meets a step of 2 or
+// more (an fp16 of which a bit of kKv4BigStep is set).
+constexpr float kKv4Top = 13.0f, kKv4BigTop = 1.0f;
+constexpr uint32_t kKv4BigStep = 0x40004000u;
 
-// Scores of one cache tile against one head block, less `base` (log2 units):
-// tokens 4q..4q+3 of head j.
-template <int KV, int D>
-__device__ __forceinline__ void kv4_scores(const Kv4Keys<D> &k, const Kv4Query<KV, D> &qr, int lane,
-                                           float base, float (&x)[4]) {
+template <int N> __device__ __forceinline__ void lds_words(const char *p, uint32_t (&w)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const u32x4 x = *(const u32x4 *)(p + 4 * i);
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[i + e] = lane_word(x, e);
+        }
+    } else if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const u32x2 x = *(const u32x2 *)(p + 4 * i);
+            w[i] = x.x;
+            w[i + 1] = x.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = *(const uint32_t *)(p + 4 * i);
+    }
+}
+
+// Scores of one cache tile (in LDS at t) against R head blocks, less each
+// block's base (log2 units): x[b][at..at+3], tokens 4q..4q+3 of head j.
+template <int KV, int D, int R>
+__device__ __forceinline__ void kv4_scores(const char *t, const Kv4Query<KV, D> (&qr)[R],
+                                           const Kv4State<D> (&st)[R], int lane, int at,
+                                           float (&x)[R][8]) {
     using G = Kv4Geometry<D>;
     constexpr int NG = G::NG;
+    const int j = lane & 15, q = lane >> 4;
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    uint32_t code[NG], step[2 * NG], low[G::kLowWords];
+    lds_words(t + kv4_k_word(NG, j, q, 0), code);
+    lds_words(t + kv4_step(NG, 4 * q, 0), step);
+    if constexpr (NG == 1) {
+        low[0] = *(const uint16_t *)(t + kv4_k_low(NG, j, 0));
+    } else if constexpr (NG == 3) {
+        low[0] = *(const uint32_t *)(t + kv4_k_low(NG, j, 0));
+        low[1] = *(const uint16_t *)(t + kv4_k_low(NG, j, 2));
+    } else {
+        lds_words(t + kv4_k_low(NG, j, 0), low);
+    }
     u32x4 a;  // lows of this lane's quarter's groups, twice (the sums' hi and lo)
     {
-        uint32_t w0 = k.low[0], w1 = G::kLowWords > 1 ? k.low[G::kLowWords > 1 ? 1 : 0] : 0u;
+        uint32_t w0 = low[0], w1 = G::kLowWords > 1 ? low[G::kLowWords > 1 ? 1 : 0] : 0u;
         if constexpr (NG > 4) {
-            const bool up = (lane >> 4) == 1;
-            w0 = up ? k.low[2] : w0;
-            w1 = up ? (G::kLowWords > 3 ? k.low[G::kLowWords > 3 ? 3 : 0] : 0u) : w1;
+            w0 = q == 1 ? low[2] : w0;
+            w1 = q == 1 ? (G::kLowWords > 3 ? low[G::kLowWords > 3 ? 3 : 0] : 0u) : w1;
         }
         a = u32x4{w0, w1, w0, w1};
     }
-    const f32x4 lows = mfma_h(a, qr.sums, zero);
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 lows[R];
+    float s[R][4];
 #pragma unroll
-    for (int g = 0; g < NG; g++) {
-        const uint32_t w = k.code[g], y = w >> 8;
-        const u32x4 c = {code_pair<false>(w), code_pair<true>(w), code_pair<false>(y), code_pair<true>(y)};
-        f32x4 t = mfma_h(c, qr.q[0][g], zero);
-        if constexpr (KV == KV_F32) t = mfma_h(c, qr.q[1][g], t);
-        const f16x2 s01 = __builtin_bit_cast(f16x2, (uint32_t)k.step[g].x);
-        const f16x2 s23 = __builtin_bit_cast(f16x2, (uint32_t)k.step[g].y);
-        s[0] = fmaf((float)s01.x, t[0], s[0]);
-        s[1] = fmaf((float)s01.y, t[1], s[1]);
-        s[2] = fmaf((float)s23.x, t[2], s[2]);
-        s[3] = fmaf((float)s23.y, t[3], s[3]);
+    for (int b = 0; b < R; b++) {
+        lows[b] = mfma_h(a, qr[b].sums, zero);
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[b][i] = 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = fmaf(qr.a, s[i], fmaf(qr.b, lows[i], -base));
+    for (int g = 0; g < NG; g++) {
+        const uint32_t w = code[g], y = w >> 8;
+        const u32x4 c = {code_pair<false>(w), code_pair<true>(w), code_pair<false>(y), code_pair<true>(y)};
+        const f16x2 s01 = __builtin_bit_cast(f16x2, step[2 * g]);
+        const f16x2 s23 = __builtin_bit_cast(f16x2, step[2 * g + 1]);
+#pragma unroll
+        for (int b = 0; b < R; b++) {
+            f32x4 d = mfma_h(c, qr[b].q[0][g], zero);
+            if constexpr (KV == KV_F32) d = mfma_h(c, qr[b].q[1][g], d);
+            s[b][0] = fmaf((float)s01.x, d[0], s[b][0]);
+            s[b][1] = fmaf((float)s01.y, d[1], s[b][1]);
+            s[b][2] = fmaf((float)s23.x, d[2], s[b][2]);
+            s[b][3] = fmaf((float)s23.y, d[3], s[b][3]);
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < R; b++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            x[b][at + i] = fmaf(qr[b].a, s[b][i], fmaf(qr[b].b, lows[b][i], -st[b].base));
 }
 
-// O += P V of one tile and head block.  pe: the weights of the lane's tokens
-// 4q..4q+3 of a, then of b.  BIG: a step of the tile is 2 or more.
-template <int KV, int D, bool BIG>
-__device__ __forceinline__ void kv4_pv(const Kv4Values<D> &va, const Kv4Values<D> &vb,
-                                       const float (&pe)[8], Kv4State<D> &st) {
+// The values of one tile, out of LDS: of a, then of b.
+template <int D> struct Kv4Values {
+    uint32_t code[2][Kv4Geometry<D>::NG];      // tokens 4q..4q+3, channel pair j of each group
+    uint32_t step[2][2 * Kv4Geometry<D>::NG];  // tokens 4q..4q+3 of each group
+    uint32_t low[2][2];                        // tokens 4q..4q+3 of group j (row NG: ones)
+};
+
+// O += P V of one tile.  pe: the weights of the lane's tokens 4q..4q+3 of a,
+// then of b.
+template <int KV, int D, int R>
+__device__ __forceinline__ void kv4_pv(const Kv4Values<D> &v, const float (&pe)[R][8], Kv4State<D> (&st)[R]) {
     constexpr int NG = Kv4Geometry<D>::NG;
     constexpr bool kLo = KV != KV_BF16;  // a second fp16 part of the weights
-    constexpr float kDown = BIG ? 1.0f / 4096.0f : 1.0f;
-    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    {
-        u32x4 hi, lo;
+    u32x4 ph[R], pl[R];
+    const u32x4 a = {v.low[0][0], v.low[0][1], v.low[1][0], v.low[1][1]};
+#pragma unroll
+    for (int b = 0; b < R; b++) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            hi[i] = half_pair(pe[2 * i], pe[2 * i + 1]);
+            const uint32_t h = half_pair(pe[b][2 * i], pe[b][2 * i + 1]);
+            ph[b][i] = h;
             if constexpr (kLo) {
-                const f32x2 r = unpack16<KV_F16>(lane_word(hi, i));
-                lo[i] = half_pair(pe[2 * i] - r.x, pe[2 * i + 1] - r.y);
+                const f32x2 r = unpack16<KV_F16>(h);
+                pl[b][i] = half_pair(pe[b][2 * i] - r.x, pe[b][2 * i + 1] - r.y);
             }
         }
-        const u32x4 a = {va.low.x, va.low.y, vb.low.x, vb.low.y};
-        st.low = mfma_h(a, hi, st.low);
-        if constexpr (kLo) st.low = mfma_h(a, lo, st.low);
+        st[b].low = mfma_h(a, ph[b], st[b].low);
+        if constexpr (kLo) st[b].low = mfma_h(a, pl[b], st[b].low);
     }
 #pragma unroll
     for (int g = 0; g < NG; g++) {
-        const uint32_t sw[4] = {va.step[g].x, va.step[g].y, vb.step[g].x, vb.step[g].y};
-        f16x8 hi, lo;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const f16x2 s = __builtin_bit_cast(f16x2, sw[i]);
-            const float w0 = BIG ? pe[2 * i] * kDown : pe[2 * i];
-            const float w1 = BIG ? pe[2 * i + 1] * kDown : pe[2 * i + 1];
-            const _Float16 h0 = (_Float16)(w0 * (float)s.x), h1 = (_Float16)(w1 * (float)s.y);
-            hi[2 * i] = h0;
-            hi[2 * i + 1] = h1;
-            if constexpr (kLo) {
-                lo[2 * i] = (_Float16)fmaf(w0, (float)s.x, -(float)h0);
-                lo[2 * i + 1] = (_Float16)fmaf(w1, (float)s.y, -(float)h1);
-            }
-        }
-        const u32x4 ph = __builtin_bit_cast(u32x4, hi), pl = __builtin_bit_cast(u32x4, lo);
-        const uint32_t x = va.code[g], x8 = x >> 8, y = vb.code[g], y8 = y >> 8;
+        const uint32_t x = v.code[0][g], x8 = x >> 8, y = v.code[1][g], y8 = y >> 8;
         const u32x4 even = {code_pair<false>(x), code_pair<false>(x8), code_pair<false>(y), code_pair<false>(y8)};
         const u32x4 odd = {code_pair<true>(x), code_pair<true>(x8), code_pair<true>(y), code_pair<true>(y8)};
-        f32x4 t0 = mfma_h(even, ph, BIG ? zero : st.o[g][0]);
-        f32x4 t1 = mfma_h(odd, ph, BIG ? zero : st.o[g][1]);
-        if constexpr (kLo) {
-            t0 = mfma_h(even, pl, t0);
-            t1 = mfma_h(odd, pl, t1);
+#pragma unroll
+        for (int b = 0; b < R; b++) {
+            u32x4 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const f16x2 s = __builtin_bit_cast(f16x2, v.step[i >> 1][2 * g + (i & 1)]);
+                const f16x2 h = __builtin_bit_cast(f16x2, lane_word(ph[b], i));
+                const f16x2 c = h * s;
+                hi[i] = __builtin_bit_cast(uint32_t, c);
+                if constexpr (kLo) {
+                    const f16x2 l = __builtin_bit_cast(f16x2, lane_word(pl[b], i));
+                    const f16x2 r = __builtin_elementwise_fma(h, s, -c);
+                    lo[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(l, s, r));
+                }
+            }
+            st[b].o[g][0] = mfma_h(even, hi, st[b].o[g][0]);
+            st[b].o[g][1] = mfma_h(odd, hi, st[b].o[g][1]);
+            if constexpr (kLo) {
+                st[b].o[g][0] = mfma_h(even, lo, st[b].o[g][0]);
+                st[b].o[g][1] = mfma_h(odd, lo, st[b].o[g][1]);
+            }
         }
-        st.o[g][0] = BIG ? st.o[g][0] + t0 * 4096.0f : t0;
-        st.o[g][1] = BIG ? st.o[g][1] + t1 * 4096.0f : t1;
     }
+}
+
+// Row r of the state's low sums (the lane's head).
+template <int D> __device__ __forceinline__ float kv4_low_row(const Kv4State<D> &st, int r, int lane) {
+    const float own = st.low[r & 3];
+    return __shfl(own, (r >> 2) * 16 + (lane & 15));
 }
 
 // The state's value of the lane's 8 channels of group g (32g + 8q..+7), not
 // yet divided by l.
 template <int D>
 __device__ __forceinline__ void kv4_channels(const Kv4State<D> &st, int g, int lane, float (&f)[8]) {
-    // the group's low sum, from its quarter
-    const float own = st.low[g & 3];
-    const float low = __shfl(own, (g >> 2) * 16 + (lane & 15));
+    const float low = kv4_low_row<D>(st, g, lane);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         f[2 * i] = fmaf(st.o[g][0][i], 16777216.0f, low);
@@ -361,9 +387,7 @@ __device__ __forceinline__ void kv4_write(const DecodeParams &p, const MfmaPiece
     const int nh = min(GT, p.group - g0);
 #pragma unroll
     for (int b = 0; b < R; b++) {
-        float l = st[b].l;
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
+        const float l = kv4_low_row<D>(st[b], NG, lane);
         const int hj = 16 * b + j;
         const float mul = !pc.whole ? 1.0f : l > 0.0f || l != l ? 1.0f / l : 0.0f;
         const size_t row = ((size_t)pc.slot * GT + hj) * D;
@@ -388,56 +412,78 @@ __device__ __forceinline__ void kv4_write(const DecodeParams &p, const MfmaPiece
     }
 }
 
-// Where a tile's two cache tiles are: page ids (negative: not there) and the
-// first token.
+// One tile of a wavefront's range: the kv head, its first token, the end of
+// its piece's tokens, and the page ids of its two cache tiles (negative: not
+// there).
 struct Kv4TileRef {
-    int t0, t_end, blk_a, blk_b;
+    int kvh, t0, t_end, blk_a, blk_b;
 };
 
+// Walks the tiles of a wavefront's range, across its pieces, ahead of the
+// computation; page ids are read (scalar loads) one tile before their use.
+struct Kv4Walker {
+    RangeCursor cur;
+    MfmaPiece pc;
+    bool more;
+    Kv4TileRef next;
+
+    __device__ __forceinline__ void ids(const DecodeParams &p, const int *__restrict__ tables) {
+        const int *bt = tables + (size_t)pc.s * p.max_blocks;
+        const int tb = next.t0 + kKv4Tile;
+        next.blk_a = bt[next.t0 >> p.bs_shift];
+        next.blk_b = tb < next.t_end ? bt[tb >> p.bs_shift] : -1;
+    }
+    __device__ __forceinline__ void piece(const DecodeParams &p, const int *__restrict__ lens,
+                                          const int *__restrict__ tables, const int *pre) {
+        more = next_piece<kKv4TileTokens>(p, lens, pre, cur, pc);
+        if (more) {
+            next = Kv4TileRef{pc.kvh, pc.t_begin, pc.t_end, -1, -1};
+            ids(p, tables);
+        }
+    }
+    __device__ __forceinline__ Kv4TileRef take(const DecodeParams &p, const int *__restrict__ lens,
+                                               const int *__restrict__ tables, const int *pre) {
+        if (!more) return Kv4TileRef{0, 0, 0, -1, -1};
+        const Kv4TileRef r = next;
+        next.t0 += kKv4TileTokens;
+        if (next.t0 < next.t_end) ids(p, tables);
+        else piece(p, lens, tables, pre);
+        return r;
+    }
+};
+
+// K (or V) of a tile into its half of an LDS slot.
 template <int D>
-__device__ __forceinline__ const char *kv4_tile_at(const DecodeParams &p, const char *base, int t, int blk) {
-    return base + (long long)blk * p.kv_block_stride +
-           (long long)((t & (p.block_size - 1)) / kKv4Tile) * Kv4Geometry<D>::kBytes;
+__device__ __forceinline__ void kv4_fetch_half(const DecodeParams &p, const void *cache,
+                                               const Kv4TileRef &r, uint32_t lds, int lane) {
+    constexpr int kBytes = Kv4Geometry<D>::kBytes;
+    const char *base = (const char *)cache + (size_t)r.kvh * (size_t)p.kv_head_stride;
+    const int mask = p.block_size - 1;
+    const char *a = base + (long long)r.blk_a * p.kv_block_stride + ((r.t0 & mask) >> 4) * kBytes;
+    const char *b = base + (long long)r.blk_b * p.kv_block_stride + (((r.t0 + 16) & mask) >> 4) * kBytes;
+    kv4_fetch<D>(a, r.blk_a >= 0, lds, lane);
+    kv4_fetch<D>(b, r.blk_b >= 0, lds + kBytes, lane);
 }
 
-template <int D>
-__device__ __forceinline__ void kv4_load_k(const DecodeParams &p, const char *kb, const Kv4TileRef &r,
-                                           int lane, Kv4Keys<D> (&k)[2]) {
-    kv4_load_keys<D>(kv4_rsrc<D>(kv4_tile_at<D>(p, kb, r.t0, r.blk_a), r.blk_a >= 0), lane, k[0]);
-    kv4_load_keys<D>(kv4_rsrc<D>(kv4_tile_at<D>(p, kb, r.t0 + 16, r.blk_b), r.blk_b >= 0), lane, k[1]);
-}
-
-template <int D>
-__device__ __forceinline__ void kv4_load_v(const DecodeParams &p, const char *vb, const Kv4TileRef &r,
-                                           int lane, Kv4Values<D> (&v)[2]) {
-    kv4_load_values<D>(kv4_rsrc<D>(kv4_tile_at<D>(p, vb, r.t0, r.blk_a), r.blk_a >= 0), lane, v[0]);
-    kv4_load_values<D>(kv4_rsrc<D>(kv4_tile_at<D>(p, vb, r.t0 + 16, r.blk_b), r.blk_b >= 0), lane, v[1]);
-}
-
-// Page ids of the piece's cache tiles first .. first + 63, lane i holding
-// cache tile first + i (past the piece's end: -1).
-__device__ __forceinline__ int kv4_load_ids(const DecodeParams &p, const int *__restrict__ tables,
-                                            const MfmaPiece &pc, int first, int lane) {
-    const int *bt = tables + (size_t)pc.s * p.max_blocks;
-    const int t = pc.t_begin + kKv4Tile * (first + lane);
-    const int id = bt[(t < pc.t_end ? t : pc.t_end - 1) >> p.bs_shift];
-    return t < pc.t_end ? id : -1;
-}
-
-// Wavefronts per SIMD the kernel is compiled for.
+// Wavefronts per SIMD the kernel is compiled for: as many as two LDS slots
+// each and the state's registers leave room for.
 constexpr int kv4_waves_per_simd(int head_size, int row_blocks) {
-    return head_size > 128 || row_blocks > 1 ? (head_size * row_blocks > 256 ? 1 : 2) : 2;
+    return head_size > 192 ? 1 : head_size > 128 || row_blocks > 1 ? 2 : 3;
 }
 
 template <int KV, int D, int R>
 __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D, R))) void paged_decode_partition_kv4_kernel(
     const DecodeParams p, const int *__restrict__ lens, const int *__restrict__ tables) {
+    using G = Kv4Geometry<D>;
+    constexpr int TT = kKv4TileTokens, NG = G::NG, NF = G::kHalfFetches;
     extern __shared__ int pre[];  // num_seqs + 1 split-unit prefixes
-    constexpr int TT = kKv4TileTokens;
+    __shared__ __attribute__((aligned(16))) char slots[kKv4Waves][2][G::kSlot];
+    __shared__ __attribute__((aligned(16))) uint32_t ones[4];
+    if (threadIdx.x < 4) ones[threadIdx.x] = 0x3C003C00u;  // 1.0, 1.0
     batch_prefix<TT, kKv4Waves>(p, pre);
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int total = pre[p.num_seqs];
+    const int total = __builtin_amdgcn_readfirstlane(pre[p.num_seqs]);
     const int w = logical_block(p, total) * kKv4Waves + wave;
     const int tpw = tiles_per_wave(total, p.num_waves, p.min_tiles_per_wave);
     if (blockIdx.x == 0 && threadIdx.x == 0) p.ws_prefix[p.num_seqs + 1] = tpw;  // for the merge
@@ -457,57 +503,58 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D, R))) void pa
         }
         cur.s = __builtin_amdgcn_readfirstlane(lo);
     }
+    Kv4Walker ahead;
+    ahead.cur = cur;
+    ahead.piece(p, lens, tables, pre);
     MfmaPiece pc;
     if (!next_piece<TT>(p, lens, pre, cur, pc)) return;
-    int ids = kv4_load_ids(p, tables, pc, 0, lane);
-    Kv4Keys<D> k[2];
-    Kv4Values<D> v[2];
-    Kv4TileRef at = {pc.t_begin, pc.t_end, __builtin_amdgcn_readlane(ids, 0), __builtin_amdgcn_readlane(ids, 1)};
-    kv4_load_k<D>(p, (const char *)p.k + (size_t)pc.kvh * p.kv_head_stride, at, lane, k);
-    kv4_load_v<D>(p, (const char *)p.v + (size_t)pc.kvh * p.kv_head_stride, at, lane, v);
-    while (true) {
+    // LDS address of the wavefront's slots, K half then V half of each
+    const uint32_t lds0 =
+        (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)&slots[0][0][0] +
+        (uint32_t)(wave * 2 * G::kSlot);
+    Kv4TileRef at = ahead.take(p, lens, tables, pre);
+    kv4_fetch_half<D>(p, p.k, at, lds0, lane);
+    kv4_fetch_half<D>(p, p.v, at, lds0 + 2 * G::kBytes, lane);
+    Kv4TileRef then = ahead.take(p, lens, tables, pre);
+    kv4_fetch_half<D>(p, p.k, then, lds0 + G::kSlot, lane);
+    kv4_fetch_half<D>(p, p.v, then, lds0 + G::kSlot + 2 * G::kBytes, lane);
+    int slot = 0;
+    bool has_next = true;
+    while (has_next) {
         Kv4Query<KV, D> qr[R];
         Kv4State<D> st[R];
         const int g0 = pc.ht * kMfmaHeads * R;
+        float top = kKv4Top;
+        uint32_t big_step = kKv4BigStep;
 #pragma unroll
         for (int b = 0; b < R; b++) {
             kv4_load_query<KV, D>(p, pc, lane, g0 + 16 * b, p.group - g0 - 16 * b, qr[b]);
 #pragma unroll
-            for (int g = 0; g < Kv4Geometry<D>::NG; g++)
-                st[b].o[g][0] = st[b].o[g][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int g = 0; g < NG; g++) st[b].o[g][0] = st[b].o[g][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             st[b].low = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            st[b].l = st[b].base = 0.0f;
+            st[b].base = 0.0f;
             st[b].limit = -INFINITY;
         }
-        MfmaPiece pn = pc;
-        const bool has_next = next_piece<TT>(p, lens, pre, cur, pn);
-        const int ids_n = kv4_load_ids(p, tables, pn, 0, lane);
-        const int ntiles = (pc.t_end - pc.t_begin + TT - 1) / TT;
-        for (int i = 0; i < ntiles; i++) {
-            // the next tile: this piece's, the next piece's first, or none
-            Kv4TileRef nx;
-            const bool in_piece = i + 1 < ntiles;
-            if (in_piece) {
-                const int n = 2 * (i + 1) & 63;
-                if (n == 0) ids = kv4_load_ids(p, tables, pc, 2 * (i + 1), lane);
-                nx = {at.t0 + TT, pc.t_end, __builtin_amdgcn_readlane(ids, n), __builtin_amdgcn_readlane(ids, n + 1)};
-            } else if (has_next) {
-                nx = {pn.t_begin, pn.t_end, __builtin_amdgcn_readlane(ids_n, 0), __builtin_amdgcn_readlane(ids_n, 1)};
-            } else {
-                nx = {0, 0, -1, -1};
-            }
-            const int kvh_n = in_piece ? pc.kvh : pn.kvh;
-
+        for (int t0 = pc.t_begin; t0 < pc.t_end; t0 += TT) {
+            const Kv4TileRef nx = ahead.take(p, lens, tables, pre);
+            const char *ks = &slots[wave][slot][0], *vs = ks + 2 * G::kBytes;
+            const uint32_t lds = lds0 + (uint32_t)(slot * G::kSlot);
             float x[R][8];
-#pragma unroll
-            for (int b = 0; b < R; b++) {
-                kv4_scores<KV, D>(k[0], qr[b], lane, st[b].base, *(float(*)[4]) & x[b][0]);
-                kv4_scores<KV, D>(k[1], qr[b], lane, st[b].base, *(float(*)[4]) & x[b][4]);
-            }
-            kv4_load_k<D>(p, (const char *)p.k + (size_t)kvh_n * p.kv_head_stride, nx, lane, k);
+            kv4_wait<3 * NF>();  // later: this tile's V, the next one's K and V
+            kv4_scores<KV, D, R>(ks, qr, st, lane, 0, x);
+            kv4_scores<KV, D, R>(ks + G::kBytes, qr, st, lane, 4, x);
+            kv4_fetch_half<D>(p, p.k, nx, lds, lane);
 
-            const int q4 = (lane >> 4) * 4;
-            const bool full = at.t0 + TT <= at.t_end && at.blk_a >= 0 && at.blk_b >= 0;
+            kv4_wait<3 * NF>();  // later: the next tile's K and V, K of the one after
+            Kv4Values<D> v;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const char *t = vs + h * G::kBytes;
+                lds_words(t + kv4_v_word(NG, q, j, 0), v.code[h]);
+                lds_words(t + kv4_step(NG, 4 * q, 0), v.step[h]);
+                lds_words(j < NG ? t + kv4_v_low(NG, 4 * q, j) : (const char *)ones, v.low[h]);
+            }
+            const bool full = t0 + TT <= at.t_end && at.blk_a >= 0 && at.blk_b >= 0;
             if (!full) {
                 // tokens past the end or in missing pages: no weight, and no
                 // step or low of theirs (whatever the slots hold) in a product
@@ -516,68 +563,68 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D, R))) void pa
                     bool ok[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        ok[e] = (h ? at.blk_b : at.blk_a) >= 0 && at.t0 + 16 * h + q4 + e < at.t_end;
+                        ok[e] = (h ? at.blk_b : at.blk_a) >= 0 && t0 + 16 * h + 4 * q + e < at.t_end;
 #pragma unroll
                         for (int b = 0; b < R; b++) x[b][4 * h + e] = ok[e] ? x[b][4 * h + e] : -INFINITY;
                     }
                     const uint32_t m01 = (ok[0] ? 0xFFFFu : 0u) | (ok[1] ? 0xFFFF0000u : 0u);
                     const uint32_t m23 = (ok[2] ? 0xFFFFu : 0u) | (ok[3] ? 0xFFFF0000u : 0u);
 #pragma unroll
-                    for (int g = 0; g < Kv4Geometry<D>::NG; g++) {
-                        v[h].step[g].x &= m01;
-                        v[h].step[g].y &= m23;
+                    for (int g = 0; g < NG; g++) {
+                        v.step[h][2 * g] &= m01;
+                        v.step[h][2 * g + 1] &= m23;
                     }
-                    v[h].low.x &= m01;
-                    v[h].low.y &= m23;
+                    v.low[h][0] &= m01;
+                    v.low[h][1] &= m23;
                 }
             }
             uint32_t steps = 0;
 #pragma unroll
-            for (int g = 0; g < Kv4Geometry<D>::NG; g++)
-                steps |= v[0].step[g].x | v[0].step[g].y | v[1].step[g].x | v[1].step[g].y;
-            const bool big = __any((steps & 0x40004000u) != 0);  // fp16: 2 or more
+            for (int g = 0; g < 2 * NG; g++) steps |= v.step[0][g] | v.step[1][g];
+            const bool big = __any((steps & big_step) != 0);
 #pragma unroll
             for (int b = 0; b < R; b++) {
                 Kv4State<D> &s = st[b];
                 float mx = x[b][0];
 #pragma unroll
                 for (int e = 1; e < 8; e++) mx = fmaxf(mx, x[b][e]);
-                if (__any(mx > s.limit)) {
+                if (big || __any(mx > s.limit)) {
+                    if (big) top = kKv4BigTop;
                     mx = fmaxf(mx, __shfl_xor(mx, 16));
                     mx = fmaxf(mx, __shfl_xor(mx, 32));
-                    const bool up = mx > s.limit;
-                    const float base = up ? s.base + (mx - kKv4Top) : s.base;
-                    const float alpha = up && s.limit != -INFINITY ? fast_exp2(s.base - base) : 1.0f;
-                    s.base = base;
-                    s.limit = up ? kKv4Top : s.limit;
-                    s.l *= alpha;
+                    const bool fresh = s.limit == -INFINITY;
+                    // this head's new base: where the larger of its old and
+                    // new largest scores has weight 2^top
+                    const float most = fmaxf(mx, s.limit);
+                    const bool any = most != -INFINITY;
+                    const float down = any ? most - top : 0.0f;
+                    const float alpha = fresh || down == 0.0f ? 1.0f : fast_exp2(-down);
+                    s.base += down;
+                    s.limit = any ? top : s.limit;
                     s.low *= alpha;
 #pragma unroll
-                    for (int g = 0; g < Kv4Geometry<D>::NG; g++) {
+                    for (int g = 0; g < NG; g++) {
                         s.o[g][0] *= alpha;
                         s.o[g][1] *= alpha;
                     }
-                    // (the largest weight is 2^13 to the bit)
+                    // (the largest weight is 2^top to the bit)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[b][e] = up ? (x[b][e] - mx) + kKv4Top : x[b][e];
+                    for (int e = 0; e < 8; e++) x[b][e] = down != 0.0f ? (x[b][e] - most) + top : x[b][e];
                 }
-                float pe[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    pe[e] = fast_exp2(x[b][e]);
-                    s.l += pe[e];
-                }
-                if (big) kv4_pv<KV, D, true>(v[0], v[1], pe, s);
-                else kv4_pv<KV, D, false>(v[0], v[1], pe, s);
+                for (int e = 0; e < 8; e++) x[b][e] = fast_exp2(x[b][e]);
             }
-            kv4_load_v<D>(p, (const char *)p.v + (size_t)kvh_n * p.kv_head_stride, nx, lane, v);
-            at = nx;
+            if (big) big_step = 0;
+            kv4_pv<KV, D, R>(v, x, st);
+            kv4_fetch_half<D>(p, p.v, nx, lds + 2 * G::kBytes, lane);
+            at = then;
+            then = nx;
+            slot ^= 1;
         }
         kv4_write<KV, D, R>(p, pc, lane, st);
-        if (!has_next) break;
-        pc = pn;
-        ids = ids_n;
+        has_next = next_piece<TT>(p, lens, pre, cur, pc);
     }
+    kv4_wait<0>();  // nothing of this wavefront's may reach LDS after its end
 }
 
 // Two row blocks per wavefront for groups of 17 to 32 heads.
