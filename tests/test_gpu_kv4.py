@@ -473,3 +473,15 @@ def test_refused_calls_leave_the_output(cuda):
         with pytest.raises(ValueError):
             call()
     assert bool((out == 7.0).all())
+
+
+def test_repeated_calls_give_the_same_bits(cuda):
+    """Many short sequences with partly filled tiles and missing pages: nothing
+    depends on when a fetch comes back."""
+    lens = [1 + (i * 7) % 90 for i in range(4000)]
+    for d, kvh in ((32, 1), (128, 2)):
+        q, k, v, kc, vc, bt = _batch("fp16", 2 * kvh, kvh, d, 16, lens, seed=3)
+        bt[::5, 0] = -1
+        want = _attend(q, kc, vc, bt, lens, kvh)
+        for _ in range(15):
+            assert torch.equal(_attend(q, kc, vc, bt, lens, kvh), want)

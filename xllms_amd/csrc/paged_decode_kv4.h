@@ -68,7 +68,8 @@ template <int D> struct Kv4Geometry {
     static constexpr int kPieces = kBytes / 16;             // 16-byte pieces of a cache tile
     static constexpr int kFetches = (kPieces + 63) / 64;    // loads of a cache tile
     static constexpr int kLowWords = (NG + 1) / 2;          // a token's lows of K
-    static constexpr int kSlot = 4 * kBytes;                // K a, K b, V a, V b
+    static constexpr int kOnes = 4 * kBytes;                // K a, K b, V a, V b, then eight ones
+    static constexpr int kSlot = 4 * kBytes + 16;
     static constexpr int kHalfFetches = 2 * kFetches;       // loads of K (or V) of a tile
 };
 
@@ -108,6 +109,21 @@ __device__ __forceinline__ f32x4 mfma_h(u32x4 a, u32x4 b, f32x4 c) {
 
 __device__ __forceinline__ uint32_t half_pair(float a, float b) { return pack16<KV_F16>(a, b); }
 
+// What fp16 pair h leaves of two floats it was rounded from, as an fp16 pair
+// (the differences are exact in fp32).
+__device__ __forceinline__ uint32_t half_rest(float a, float b, uint32_t h) {
+    uint32_t r;
+    asm("v_fma_mixlo_f16 %0, %1, 1.0, -%2 op_sel_hi:[0,0,1]" : "=v"(r) : "v"(a), "v"(h));
+    asm("v_fma_mixhi_f16 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(r) : "v"(b), "v"(h));
+    return r;
+}
+
+// x where ok, else -inf: in place, inside a rarely taken branch.
+__device__ __forceinline__ void keep_score(float &x, bool ok) {
+    const unsigned long long m = __ballot(ok);
+    asm("v_cndmask_b32 %0, %1, %0, %2" : "+v"(x) : "v"(-INFINITY), "s"(m));
+}
+
 // Two codes of a word as fp16: nibbles 0 and 4 (times 2^-24), or with HIGH
 // nibbles 1 and 5 (times 2^-20).
 template <bool HIGH> __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
@@ -118,7 +134,8 @@ template <bool HIGH> __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
 template <int KV, int D> struct Kv4Query {
     static constexpr int kTerms = KV == KV_F32 ? 2 : 1;
     u32x4 q[kTerms][Kv4Geometry<D>::NG];
-    u32x4 sums;        // the groups' sums: quarter q's 4 groups, hi and lo
+    u32x2 sums;        // the groups' sums, in fp16 parts hi (quarters 0, 1: groups 0-3,
+                       // 4-7) and lo (quarters 2, 3)
     float a, b;        // score (log2 units) = a * (code part) + b * (low part)
 };
 
@@ -185,20 +202,19 @@ __device__ __forceinline__ void kv4_load_query(const DecodeParams &p, const Mfma
             o.q[1][g] = lo;
         }
     }
-    // Quarter q < 2 holds groups 4q..4q+3; the other quarters nothing.  A query
-    // with an infinity or NaN makes every score of its head NaN.
+    // A query with an infinity or NaN makes every score of its head NaN.
+    if (row_bad) sum[0] = __builtin_nanf("");
     float s4[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const float s0 = i < NG ? sum[i < NG ? i : 0] : 0.0f;
         const float s1 = 4 + i < NG ? sum[4 + i < NG ? 4 + i : 0] : 0.0f;
-        s4[i] = q == 0 ? s0 : q == 1 ? s1 : 0.0f;
+        s4[i] = q & 1 ? s1 : s0;
     }
-    if (row_bad && q == 0) s4[0] = __builtin_nanf("");
     const uint32_t h01 = half_pair(s4[0], s4[1]), h23 = half_pair(s4[2], s4[3]);
     const f32x2 r01 = unpack16<KV_F16>(h01), r23 = unpack16<KV_F16>(h23);
-    o.sums = u32x4{h01, h23, half_pair(s4[0] - r01.x, s4[1] - r01.y),
-                   half_pair(s4[2] - r23.x, s4[3] - r23.y)};
+    o.sums = q < 2 ? u32x2{h01, h23}
+                   : u32x2{half_pair(s4[0] - r01.x, s4[1] - r01.y), half_pair(s4[2] - r23.x, s4[3] - r23.y)};
     o.a = __builtin_amdgcn_ldexpf(p.scale_log2, ex - 15 + 24);
     o.b = __builtin_amdgcn_ldexpf(p.scale_log2, ex - 15 + 9);
 }
@@ -260,20 +276,17 @@ __device__ __forceinline__ void kv4_scores(const char *t, const Kv4Query<KV, D> 
     } else {
         lds_words(t + kv4_k_low(NG, j, 0), low);
     }
-    u32x4 a;  // lows of this lane's quarter's groups, twice (the sums' hi and lo)
-    {
-        uint32_t w0 = low[0], w1 = G::kLowWords > 1 ? low[G::kLowWords > 1 ? 1 : 0] : 0u;
-        if constexpr (NG > 4) {
-            w0 = q == 1 ? low[2] : w0;
-            w1 = q == 1 ? (G::kLowWords > 3 ? low[G::kLowWords > 3 ? 3 : 0] : 0u) : w1;
-        }
-        a = u32x4{w0, w1, w0, w1};
+    // lows of this lane's quarter's groups
+    u32x2 a = {low[0], G::kLowWords > 1 ? low[G::kLowWords > 1 ? 1 : 0] : 0u};
+    if constexpr (NG > 4) {
+        a.x = q & 1 ? low[2] : a.x;
+        a.y = q & 1 ? (G::kLowWords > 3 ? low[G::kLowWords > 3 ? 3 : 0] : 0u) : a.y;
     }
     f32x4 lows[R];
     float s[R][4];
 #pragma unroll
     for (int b = 0; b < R; b++) {
-        lows[b] = mfma_h(a, qr[b].sums, zero);
+        lows[b] = mfma_pv<KV_F16>(a, qr[b].sums, zero);
 #pragma unroll
         for (int i = 0; i < 4; i++) s[b][i] = 0.0f;
     }
@@ -322,8 +335,7 @@ __device__ __forceinline__ void kv4_pv(const Kv4Values<D> &v, const float (&pe)[
             const uint32_t h = half_pair(pe[b][2 * i], pe[b][2 * i + 1]);
             ph[b][i] = h;
             if constexpr (kLo) {
-                const f32x2 r = unpack16<KV_F16>(h);
-                pl[b][i] = half_pair(pe[b][2 * i] - r.x, pe[b][2 * i + 1] - r.y);
+                pl[b][i] = half_rest(pe[b][2 * i], pe[b][2 * i + 1], h);
             }
         }
         st[b].low = mfma_h(a, ph[b], st[b].low);
@@ -412,57 +424,60 @@ __device__ __forceinline__ void kv4_write(const DecodeParams &p, const MfmaPiece
     }
 }
 
-// One tile of a wavefront's range: the kv head, its first token, the end of
-// its piece's tokens, and the page ids of its two cache tiles (negative: not
-// there).
+// One tile of a wavefront's range: where its two cache tiles are, in bytes from
+// the start of either cache, and whether their pages are there.
 struct Kv4TileRef {
-    int kvh, t0, t_end, blk_a, blk_b;
+    long long at_a, at_b;
+    bool a, b;
 };
 
 // Walks the tiles of a wavefront's range, across its pieces, ahead of the
 // computation; page ids are read (scalar loads) one tile before their use.
-struct Kv4Walker {
+template <int D> struct Kv4Walker {
     RangeCursor cur;
     MfmaPiece pc;
     bool more;
-    Kv4TileRef next;
+    int t0, blk_a, blk_b;  // the next tile: its first token and page ids
 
     __device__ __forceinline__ void ids(const DecodeParams &p, const int *__restrict__ tables) {
         const int *bt = tables + (size_t)pc.s * p.max_blocks;
-        const int tb = next.t0 + kKv4Tile;
-        next.blk_a = bt[next.t0 >> p.bs_shift];
-        next.blk_b = tb < next.t_end ? bt[tb >> p.bs_shift] : -1;
+        const int tb = t0 + kKv4Tile;
+        blk_a = bt[t0 >> p.bs_shift];
+        blk_b = tb < pc.t_end ? bt[tb >> p.bs_shift] : -1;
     }
     __device__ __forceinline__ void piece(const DecodeParams &p, const int *__restrict__ lens,
                                           const int *__restrict__ tables, const int *pre) {
         more = next_piece<kKv4TileTokens>(p, lens, pre, cur, pc);
         if (more) {
-            next = Kv4TileRef{pc.kvh, pc.t_begin, pc.t_end, -1, -1};
+            t0 = pc.t_begin;
             ids(p, tables);
         }
     }
     __device__ __forceinline__ Kv4TileRef take(const DecodeParams &p, const int *__restrict__ lens,
                                                const int *__restrict__ tables, const int *pre) {
-        if (!more) return Kv4TileRef{0, 0, 0, -1, -1};
-        const Kv4TileRef r = next;
-        next.t0 += kKv4TileTokens;
-        if (next.t0 < next.t_end) ids(p, tables);
+        if (!more) return Kv4TileRef{0, 0, false, false};
+        constexpr unsigned kBytes = Kv4Geometry<D>::kBytes;
+        const unsigned mask = (unsigned)p.block_size - 1;
+        const long long head = (long long)pc.kvh * p.kv_head_stride;
+        const Kv4TileRef r = {
+            head + (long long)blk_a * p.kv_block_stride + ((((unsigned)t0 & mask) >> 4) * kBytes),
+            head + (long long)blk_b * p.kv_block_stride + ((((unsigned)t0 + 16 & mask) >> 4) * kBytes),
+            blk_a >= 0, blk_b >= 0};
+        t0 += kKv4TileTokens;
+        if (t0 < pc.t_end) ids(p, tables);
         else piece(p, lens, tables, pre);
         return r;
     }
 };
 
-// K (or V) of a tile into its half of an LDS slot.
+// K (or V) of a tile into its half of an LDS slot.  Every LDS access so far has
+// to be through: reads of the slot's last tile may be in the queue still, their
+// uses scheduled past this point, and a page that is not there writes at once.
 template <int D>
-__device__ __forceinline__ void kv4_fetch_half(const DecodeParams &p, const void *cache,
-                                               const Kv4TileRef &r, uint32_t lds, int lane) {
-    constexpr int kBytes = Kv4Geometry<D>::kBytes;
-    const char *base = (const char *)cache + (size_t)r.kvh * (size_t)p.kv_head_stride;
-    const int mask = p.block_size - 1;
-    const char *a = base + (long long)r.blk_a * p.kv_block_stride + ((r.t0 & mask) >> 4) * kBytes;
-    const char *b = base + (long long)r.blk_b * p.kv_block_stride + (((r.t0 + 16) & mask) >> 4) * kBytes;
-    kv4_fetch<D>(a, r.blk_a >= 0, lds, lane);
-    kv4_fetch<D>(b, r.blk_b >= 0, lds + kBytes, lane);
+__device__ __forceinline__ void kv4_fetch_half(const void *cache, const Kv4TileRef &r, uint32_t lds, int lane) {
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    kv4_fetch<D>((const char *)cache + r.at_a, r.a, lds, lane);
+    kv4_fetch<D>((const char *)cache + r.at_b, r.b, lds + Kv4Geometry<D>::kBytes, lane);
 }
 
 // Wavefronts per SIMD the kernel is compiled for: as many as two LDS slots
@@ -478,8 +493,9 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D, R))) void pa
     constexpr int TT = kKv4TileTokens, NG = G::NG, NF = G::kHalfFetches;
     extern __shared__ int pre[];  // num_seqs + 1 split-unit prefixes
     __shared__ __attribute__((aligned(16))) char slots[kKv4Waves][2][G::kSlot];
-    __shared__ __attribute__((aligned(16))) uint32_t ones[4];
-    if (threadIdx.x < 4) ones[threadIdx.x] = 0x3C003C00u;  // 1.0, 1.0
+    if (threadIdx.x < 2 * kKv4Waves)  // (the fetches leave them alone)
+        *(u32x4 *)&slots[threadIdx.x >> 1][threadIdx.x & 1][G::kOnes] =
+            u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
     batch_prefix<TT, kKv4Waves>(p, pre);
     const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -503,7 +519,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D, R))) void pa
         }
         cur.s = __builtin_amdgcn_readfirstlane(lo);
     }
-    Kv4Walker ahead;
+    Kv4Walker<D> ahead;
     ahead.cur = cur;
     ahead.piece(p, lens, tables, pre);
     MfmaPiece pc;
@@ -513,11 +529,14 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D, R))) void pa
         (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)&slots[0][0][0] +
         (uint32_t)(wave * 2 * G::kSlot);
     Kv4TileRef at = ahead.take(p, lens, tables, pre);
-    kv4_fetch_half<D>(p, p.k, at, lds0, lane);
-    kv4_fetch_half<D>(p, p.v, at, lds0 + 2 * G::kBytes, lane);
+    kv4_fetch_half<D>(p.k, at, lds0, lane);
+    kv4_fetch_half<D>(p.v, at, lds0 + 2 * G::kBytes, lane);
     Kv4TileRef then = ahead.take(p, lens, tables, pre);
-    kv4_fetch_half<D>(p, p.k, then, lds0 + G::kSlot, lane);
-    kv4_fetch_half<D>(p, p.v, then, lds0 + G::kSlot + 2 * G::kBytes, lane);
+    kv4_fetch_half<D>(p.k, then, lds0 + G::kSlot, lane);
+    kv4_fetch_half<D>(p.v, then, lds0 + G::kSlot + 2 * G::kBytes, lane);
+    // the lane's lows of V: group j's, or past the groups the ones
+    const int low_a = j < NG ? 2 * G::kBytes + kv4_v_low(NG, 4 * q, j < NG ? j : 0) : G::kOnes;
+    const int low_b = j < NG ? low_a + G::kBytes : G::kOnes;
     int slot = 0;
     bool has_next = true;
     while (has_next) {
@@ -543,40 +562,38 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D, R))) void pa
             kv4_wait<3 * NF>();  // later: this tile's V, the next one's K and V
             kv4_scores<KV, D, R>(ks, qr, st, lane, 0, x);
             kv4_scores<KV, D, R>(ks + G::kBytes, qr, st, lane, 4, x);
-            kv4_fetch_half<D>(p, p.k, nx, lds, lane);
+            kv4_fetch_half<D>(p.k, nx, lds, lane);
 
             kv4_wait<3 * NF>();  // later: the next tile's K and V, K of the one after
+            // (uniform, which the compiler cannot see)
+            if (__builtin_amdgcn_readfirstlane(t0 + TT > pc.t_end || !at.a || !at.b)) {
+                // tokens past the end or in missing pages: no weight, and no
+                // step or low of theirs (whatever the slots hold) in a product.
+                // In LDS, not in the registers: there the other way through
+                // the branch got a copy of every value.
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int n = (h ? at.b : at.a) ? pc.t_end - t0 - 16 * h : 0;  // tokens
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+#pragma unroll
+                        for (int b = 0; b < R; b++) keep_score(x[b][4 * h + e], 4 * q + e < n);
+                    uint16_t *t = (uint16_t *)(slots[wave][slot] + (2 + h) * G::kBytes);
+                    for (int i = lane; i < 16 * NG; i += 64) {
+                        if ((i / (4 * NG)) * 4 + (i & 3) < n) continue;
+                        t[kv4_step(NG, 0, 0) / 2 + i] = 0;
+                        t[kv4_v_low(NG, 0, 0) / 2 + i] = 0;
+                    }
+                }
+                wave_lds_fence();  // before the reads below, by other lanes
+            }
             Kv4Values<D> v;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const char *t = vs + h * G::kBytes;
                 lds_words(t + kv4_v_word(NG, q, j, 0), v.code[h]);
                 lds_words(t + kv4_step(NG, 4 * q, 0), v.step[h]);
-                lds_words(j < NG ? t + kv4_v_low(NG, 4 * q, j) : (const char *)ones, v.low[h]);
-            }
-            const bool full = t0 + TT <= at.t_end && at.blk_a >= 0 && at.blk_b >= 0;
-            if (!full) {
-                // tokens past the end or in missing pages: no weight, and no
-                // step or low of theirs (whatever the slots hold) in a product
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    bool ok[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        ok[e] = (h ? at.blk_b : at.blk_a) >= 0 && t0 + 16 * h + 4 * q + e < at.t_end;
-#pragma unroll
-                        for (int b = 0; b < R; b++) x[b][4 * h + e] = ok[e] ? x[b][4 * h + e] : -INFINITY;
-                    }
-                    const uint32_t m01 = (ok[0] ? 0xFFFFu : 0u) | (ok[1] ? 0xFFFF0000u : 0u);
-                    const uint32_t m23 = (ok[2] ? 0xFFFFu : 0u) | (ok[3] ? 0xFFFF0000u : 0u);
-#pragma unroll
-                    for (int g = 0; g < NG; g++) {
-                        v.step[h][2 * g] &= m01;
-                        v.step[h][2 * g + 1] &= m23;
-                    }
-                    v.low[h][0] &= m01;
-                    v.low[h][1] &= m23;
-                }
+                lds_words(ks + (h ? low_b : low_a), v.low[h]);
             }
             uint32_t steps = 0;
 #pragma unroll
@@ -616,7 +633,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D, R))) void pa
             }
             if (big) big_step = 0;
             kv4_pv<KV, D, R>(v, x, st);
-            kv4_fetch_half<D>(p, p.v, nx, lds + 2 * G::kBytes, lane);
+            kv4_fetch_half<D>(p.v, nx, lds + 2 * G::kBytes, lane);
             at = then;
             then = nx;
             slot ^= 1;
