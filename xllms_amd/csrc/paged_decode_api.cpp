@@ -1177,9 +1177,9 @@ int kv4_attention_run(void *out, const void *query, const void *key_cache, const
     for (int s0 = 0; s0 < num_seqs; s0 += per_launch) {
         const int nseq = num_seqs - s0 < per_launch ? num_seqs - s0 : per_launch;
         const size_t lds = (size_t)(nseq + 1) * sizeof(int);
-        const int occ = dtype == NXT_KV_FP16   ? xhip::kv4_occupancy_f16(head_size, head_tile, lds)
-                        : dtype == NXT_KV_BF16 ? xhip::kv4_occupancy_bf16(head_size, head_tile, lds)
-                                               : xhip::kv4_occupancy_f32(head_size, head_tile, lds);
+        const int occ = dtype == NXT_KV_FP16   ? xhip::kv4_occupancy_f16(head_size, head_tile, group, lds)
+                        : dtype == NXT_KV_BF16 ? xhip::kv4_occupancy_bf16(head_size, head_tile, group, lds)
+                                               : xhip::kv4_occupancy_f32(head_size, head_tile, group, lds);
         if (occ <= 0)
             return set_status(NXT_ATTN_E_HIP, "no occupancy for head_size %d %s", head_size,
                               dtype_name(dtype));
@@ -1211,6 +1211,7 @@ int kv4_attention_run(void *out, const void *query, const void *key_cache, const
         p.seg_cost = kKv4SegmentCost;
         p.segment_split = 1;
         p.merge_per_segment = merge_per_segment(group, head_tile, head_size, nseq, segs, cus);
+        p.wg_trace = t_wg_trace;
         const auto launch = dtype == NXT_KV_FP16   ? xhip::launch_kv4_f16
                             : dtype == NXT_KV_BF16 ? xhip::launch_kv4_bf16
                                                    : xhip::launch_kv4_f32;

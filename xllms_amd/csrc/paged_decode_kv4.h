@@ -31,10 +31,10 @@
 //     channel 32g + 2i (+ 1), so a lane ends with 8 neighbouring channels of
 //     each group.  The second sum is one more MFMA, A = lows (lane: group j), of
 //     which row NG is ones: the sum of the weights as they went in.
-//     Weights are scaled by 2^13, which keeps p * step clear of fp16's
+//     Weights are scaled to at most 2^13, which keeps p * step clear of fp16's
 //     subnormals: at 2^13 a step of up to 2 (values that span 30) leaves
 //     p * step below 2^14.  Once a piece meets a larger step its weights are
-//     scaled by 2 instead (steps end at 8734).
+//     scaled to at most 2^2 instead (steps end at 8734).
 //     p and p * step go in as two fp16 parts, hi + lo (~22 bits), by packed
 //     arithmetic: c = fp16(p_hi step), lo = fp16(p_lo step + (p_hi step - c)),
 //     the difference exact in one fma; for a bf16 output, whose half step is
@@ -89,10 +89,21 @@ __device__ __forceinline__ void kv4_fetch(const char *tile, bool ok, uint32_t ld
     const uint32_t off = (uint32_t)lane * 16;
 #pragma unroll
     for (int c = 0; c < G::kFetches; c++) {
-        if (64 * c + 64 <= G::kPieces || lane < G::kPieces - 64 * c)
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen offset:%3 nt lds"
+        constexpr int kLast = G::kPieces - 64 * (G::kFetches - 1);  // lanes of the last load
+        if (c < G::kFetches - 1 || kLast == 64)
+            asm volatile("s_mov_b32 m0, %0\n\t"
+                         "s_nop 0\n\t"
+                         "buffer_load_dwordx4 %1, %2, 0 offen offset:%3 nt lds"
                          :
                          : "s"(lds), "v"(off), "s"(rsrc), "n"(1024 * c)
+                         : "memory", "m0");
+        else  // (every lane is active here; a branch would end the scheduler's block)
+            asm volatile("s_mov_b32 m0, %0\n\t"
+                         "s_bfm_b64 exec, %4, 0\n\t"
+                         "buffer_load_dwordx4 %1, %2, 0 offen offset:%3 nt lds\n\t"
+                         "s_mov_b64 exec, -1"
+                         :
+                         : "s"(lds), "v"(off), "s"(rsrc), "n"(1024 * c), "n"(kLast)
                          : "memory", "m0");
     }
 }
@@ -131,20 +142,29 @@ template <bool HIGH> __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
 }
 
 // Query operands of one head block.  kTerms: fp16 parts of a query element.
-template <int KV, int D> struct Kv4Query {
+// SPLIT: head j & 7 in columns j and j + 8, and the operands of the two cache
+// tiles: [0] is zero in columns 8-15, [1] in columns 0-7.
+template <int KV, int D, bool SPLIT> struct Kv4Query {
     static constexpr int kTerms = KV == KV_F32 ? 2 : 1;
-    u32x4 q[kTerms][Kv4Geometry<D>::NG];
-    u32x2 sums;        // the groups' sums, in fp16 parts hi (quarters 0, 1: groups 0-3,
+    static constexpr int kTiles = SPLIT ? 2 : 1;
+    u32x4 q[kTiles][kTerms][Kv4Geometry<D>::NG];
+    u32x2 sums[kTiles];  // the groups' sums, in fp16 parts hi (quarters 0, 1: groups 0-3,
                        // 4-7) and lo (quarters 2, 3)
     float a, b;        // score (log2 units) = a * (code part) + b * (low part)
 };
 
-template <int KV, int D>
+template <int KV, int D, bool SPLIT>
 __device__ __forceinline__ void kv4_load_query(const DecodeParams &p, const MfmaPiece &pc, int lane,
-                                               int head0, int heads, Kv4Query<KV, D> &o) {
+                                               int head0, int heads, Kv4Query<KV, D, SPLIT> &o) {
     using G = Kv4Geometry<D>;
     constexpr int NG = G::NG, EB = KvTraits<KV>::kBytes;
-    const int j = lane & 15, q = lane >> 4;
+    const int j = lane & (SPLIT ? 7 : 15), q = lane >> 4;
+    // in SPLIT, the operand of one cache tile
+    const uint32_t first = !SPLIT || (lane & 8) == 0 ? ~0u : 0u;
+    auto put = [&](u32x4 *to, u32x4 x) {  // to[tile * kTerms * NG]
+        to[0] = x & first;
+        if constexpr (SPLIT) to[Kv4Query<KV, D, SPLIT>::kTerms * NG] = x & ~first;
+    };
     float x[NG][8];
     float top = 0.0f;
     bool finite = true;
@@ -173,7 +193,7 @@ __device__ __forceinline__ void kv4_load_query(const DecodeParams &p, const Mfma
     top = fmaxf(top, __shfl_xor(top, 32));
     // every quarter of the head
     const unsigned long long bad = __ballot(!finite);
-    const bool row_bad = ((bad | bad >> 16 | bad >> 32 | bad >> 48) >> j & 1) != 0;
+    const bool row_bad = ((bad | bad >> 16 | bad >> 32 | bad >> 48) >> (lane & 15) & 1) != 0;
     const int ex = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
     float sum[NG];
 #pragma unroll
@@ -191,7 +211,7 @@ __device__ __forceinline__ void kv4_load_query(const DecodeParams &p, const Mfma
         u32x4 hi;
 #pragma unroll
         for (int e = 0; e < 4; e++) hi[e] = half_pair(x[g][2 * e], x[g][2 * e + 1]);
-        o.q[0][g] = hi;
+        put(&o.q[0][0][g], hi);
         if constexpr (KV == KV_F32) {
             u32x4 lo;
 #pragma unroll
@@ -199,7 +219,7 @@ __device__ __forceinline__ void kv4_load_query(const DecodeParams &p, const Mfma
                 const f32x2 r = unpack16<KV_F16>(lane_word(hi, e));
                 lo[e] = half_pair(x[g][2 * e] - r.x, x[g][2 * e + 1] - r.y);
             }
-            o.q[1][g] = lo;
+            put(&o.q[0][1][g], lo);
         }
     }
     // A query with an infinity or NaN makes every score of its head NaN.
@@ -213,8 +233,10 @@ __device__ __forceinline__ void kv4_load_query(const DecodeParams &p, const Mfma
     }
     const uint32_t h01 = half_pair(s4[0], s4[1]), h23 = half_pair(s4[2], s4[3]);
     const f32x2 r01 = unpack16<KV_F16>(h01), r23 = unpack16<KV_F16>(h23);
-    o.sums = q < 2 ? u32x2{h01, h23}
-                   : u32x2{half_pair(s4[0] - r01.x, s4[1] - r01.y), half_pair(s4[2] - r23.x, s4[3] - r23.y)};
+    const u32x2 sums = q < 2 ? u32x2{h01, h23}
+                             : u32x2{half_pair(s4[0] - r01.x, s4[1] - r01.y), half_pair(s4[2] - r23.x, s4[3] - r23.y)};
+    o.sums[0] = sums & first;
+    if constexpr (SPLIT) o.sums[1] = sums & ~first;
     o.a = __builtin_amdgcn_ldexpf(p.scale_log2, ex - 15 + 24);
     o.b = __builtin_amdgcn_ldexpf(p.scale_log2, ex - 15 + 9);
 }
@@ -225,13 +247,15 @@ template <int D> struct Kv4State {
     f32x4 low;                       // row 4q + i: group 4q + i's sum of p * low; row NG: the
                                      // sum of p
     float base;                      // weights of head j are 2^(score - base)
-    float limit;                     // score - base up to which they are kept: `top`; -inf
-                                     // (and base 0) before the head's first score
+    float limit;                     // score - base from which the base moves; -inf (and
+                                     // base 0) before the head's first score
 };
 
-// log2 of the largest weight, before and after a piece meets a step of 2 or
-// more (an fp16 of which a bit of kKv4BigStep is set).
-constexpr float kKv4Top = 13.0f, kKv4BigTop = 1.0f;
+// log2 of the largest weight a base lets through, before and after a piece
+// meets a step of 2 or more (an fp16 of which a bit of kKv4BigStep is set).  A
+// base that moves leaves the largest score kKv4Slack below it, so that the next
+// few larger ones move nothing.
+constexpr float kKv4Limit = 13.0f, kKv4BigLimit = 2.0f, kKv4Slack = 3.0f;
 constexpr uint32_t kKv4BigStep = 0x40004000u;
 
 template <int N> __device__ __forceinline__ void lds_words(const char *p, uint32_t (&w)[N]) {
@@ -255,19 +279,19 @@ template <int N> __device__ __forceinline__ void lds_words(const char *p, uint32
     }
 }
 
-// Scores of one cache tile (in LDS at t) against R head blocks, less each
-// block's base (log2 units): x[b][at..at+3], tokens 4q..4q+3 of head j.
-template <int KV, int D, int R>
-__device__ __forceinline__ void kv4_scores(const char *t, const Kv4Query<KV, D> (&qr)[R],
-                                           const Kv4State<D> (&st)[R], int lane, int at,
-                                           float (&x)[R][8]) {
+// What a lane's scores take of one cache tile's keys, out of LDS at t: the words
+// of token j in quarter q, and its lows.
+template <int D> struct Kv4Keys {
+    uint32_t code[Kv4Geometry<D>::NG];
+    u32x2 low;  // of this lane's quarter's groups
+};
+
+template <int D> __device__ __forceinline__ void kv4_keys(const char *t, int lane, Kv4Keys<D> &k) {
     using G = Kv4Geometry<D>;
     constexpr int NG = G::NG;
     const int j = lane & 15, q = lane >> 4;
-    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    uint32_t code[NG], step[2 * NG], low[G::kLowWords];
-    lds_words(t + kv4_k_word(NG, j, q, 0), code);
-    lds_words(t + kv4_step(NG, 4 * q, 0), step);
+    uint32_t low[G::kLowWords];
+    lds_words(t + kv4_k_word(NG, j, q, 0), k.code);
     if constexpr (NG == 1) {
         low[0] = *(const uint16_t *)(t + kv4_k_low(NG, j, 0));
     } else if constexpr (NG == 3) {
@@ -276,41 +300,65 @@ __device__ __forceinline__ void kv4_scores(const char *t, const Kv4Query<KV, D> 
     } else {
         lds_words(t + kv4_k_low(NG, j, 0), low);
     }
-    // lows of this lane's quarter's groups
-    u32x2 a = {low[0], G::kLowWords > 1 ? low[G::kLowWords > 1 ? 1 : 0] : 0u};
+    k.low = u32x2{low[0], G::kLowWords > 1 ? low[G::kLowWords > 1 ? 1 : 0] : 0u};
     if constexpr (NG > 4) {
-        a.x = q & 1 ? low[2] : a.x;
-        a.y = q & 1 ? (G::kLowWords > 3 ? low[G::kLowWords > 3 ? 3 : 0] : 0u) : a.y;
+        k.low.x = q & 1 ? low[2] : k.low.x;
+        k.low.y = q & 1 ? (G::kLowWords > 3 ? low[G::kLowWords > 3 ? 3 : 0] : 0u) : k.low.y;
     }
-    f32x4 lows[R];
-    float s[R][4];
+}
+
+// The product of group g's codes of a cache tile with an operand set of a query
+// block, added to c.
+template <int KV, int D, bool SPLIT>
+__device__ __forceinline__ f32x4 kv4_group(const Kv4Keys<D> &k, int g, const Kv4Query<KV, D, SPLIT> &qr,
+                                           int tile, f32x4 c) {
+    const uint32_t w = k.code[g], y = w >> 8;
+    const u32x4 a = {code_pair<false>(w), code_pair<true>(w), code_pair<false>(y), code_pair<true>(y)};
+    c = mfma_h(a, qr.q[tile][0][g], c);
+    if constexpr (KV == KV_F32) c = mfma_h(a, qr.q[tile][1][g], c);
+    return c;
+}
+
+// Scores of a tile's cache tiles (a at t, b behind it) against R head blocks,
+// less each block's base (log2 units): x[b][0..3] of a's tokens 4q..4q+3 and
+// x[b][4..7] of b's, head j.  SPLIT: x[b][0..3] of a in columns 0-7 and of b in
+// columns 8-15.
+template <int KV, int D, int R, bool SPLIT>
+__device__ __forceinline__ void kv4_scores(const char *t, const Kv4Query<KV, D, SPLIT> (&qr)[R],
+                                           const Kv4State<D> (&st)[R], int lane,
+                                           float (&x)[R][SPLIT ? 4 : 8]) {
+    using G = Kv4Geometry<D>;
+    constexpr int NG = G::NG;
+    const int q = lane >> 4;
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    Kv4Keys<D> k[2];
+    kv4_keys<D>(t, lane, k[0]);
+    kv4_keys<D>(t + G::kBytes, lane, k[1]);
 #pragma unroll
-    for (int b = 0; b < R; b++) {
-        lows[b] = mfma_pv<KV_F16>(a, qr[b].sums, zero);
-#pragma unroll
-        for (int i = 0; i < 4; i++) s[b][i] = 0.0f;
-    }
-#pragma unroll
-    for (int g = 0; g < NG; g++) {
-        const uint32_t w = code[g], y = w >> 8;
-        const u32x4 c = {code_pair<false>(w), code_pair<true>(w), code_pair<false>(y), code_pair<true>(y)};
-        const f16x2 s01 = __builtin_bit_cast(f16x2, step[2 * g]);
-        const f16x2 s23 = __builtin_bit_cast(f16x2, step[2 * g + 1]);
+    for (int h = 0; h < (SPLIT ? 1 : 2); h++) {
+        uint32_t step[2 * NG];
+        lds_words(t + (SPLIT ? (lane & 8 ? G::kBytes : 0) : h * G::kBytes) + kv4_step(NG, 4 * q, 0), step);
 #pragma unroll
         for (int b = 0; b < R; b++) {
-            f32x4 d = mfma_h(c, qr[b].q[0][g], zero);
-            if constexpr (KV == KV_F32) d = mfma_h(c, qr[b].q[1][g], d);
-            s[b][0] = fmaf((float)s01.x, d[0], s[b][0]);
-            s[b][1] = fmaf((float)s01.y, d[1], s[b][1]);
-            s[b][2] = fmaf((float)s23.x, d[2], s[b][2]);
-            s[b][3] = fmaf((float)s23.y, d[3], s[b][3]);
+            f32x4 lows = mfma_pv<KV_F16>(k[h].low, qr[b].sums[0], zero);
+            if constexpr (SPLIT) lows = mfma_pv<KV_F16>(k[1].low, qr[b].sums[SPLIT ? 1 : 0], lows);
+            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                f32x4 d = kv4_group<KV, D, SPLIT>(k[h], g, qr[b], 0, zero);
+                if constexpr (SPLIT) d = kv4_group<KV, D, SPLIT>(k[1], g, qr[b], SPLIT ? 1 : 0, d);
+                const f16x2 s01 = __builtin_bit_cast(f16x2, step[2 * g]);
+                const f16x2 s23 = __builtin_bit_cast(f16x2, step[2 * g + 1]);
+                s[0] = fmaf((float)s01.x, d[0], s[0]);
+                s[1] = fmaf((float)s01.y, d[1], s[1]);
+                s[2] = fmaf((float)s23.x, d[2], s[2]);
+                s[3] = fmaf((float)s23.y, d[3], s[3]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                x[b][4 * h + i] = fmaf(qr[b].a, s[i], fmaf(qr[b].b, lows[i], -st[b].base));
         }
     }
-#pragma unroll
-    for (int b = 0; b < R; b++)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            x[b][at + i] = fmaf(qr[b].a, s[b][i], fmaf(qr[b].b, lows[b][i], -st[b].base));
 }
 
 // The values of one tile, out of LDS: of a, then of b.
@@ -320,10 +368,17 @@ template <int D> struct Kv4Values {
     uint32_t low[2][2];                        // tokens 4q..4q+3 of group j (row NG: ones)
 };
 
+// The word of the lane 8 columns on (j ^ 8).
+__device__ __forceinline__ uint32_t other_half(uint32_t w) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x128, 0xF, 0xF, false);  // row_ror:8
+}
+
 // O += P V of one tile.  pe: the weights of the lane's tokens 4q..4q+3 of a,
-// then of b.
-template <int KV, int D, int R>
-__device__ __forceinline__ void kv4_pv(const Kv4Values<D> &v, const float (&pe)[R][8], Kv4State<D> (&st)[R]) {
+// then of b.  SPLIT: of a in columns 0-7, which take b's from columns 8-15
+// (whose own sums are of no use).
+template <int KV, int D, int R, bool SPLIT>
+__device__ __forceinline__ void kv4_pv(const Kv4Values<D> &v, const float (&pe)[R][SPLIT ? 4 : 8],
+                                       Kv4State<D> (&st)[R]) {
     constexpr int NG = Kv4Geometry<D>::NG;
     constexpr bool kLo = KV != KV_BF16;  // a second fp16 part of the weights
     u32x4 ph[R], pl[R];
@@ -331,11 +386,13 @@ __device__ __forceinline__ void kv4_pv(const Kv4Values<D> &v, const float (&pe)[
 #pragma unroll
     for (int b = 0; b < R; b++) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < (SPLIT ? 2 : 4); i++) {
             const uint32_t h = half_pair(pe[b][2 * i], pe[b][2 * i + 1]);
             ph[b][i] = h;
+            if constexpr (SPLIT) ph[b][i + 2] = other_half(h);
             if constexpr (kLo) {
                 pl[b][i] = half_rest(pe[b][2 * i], pe[b][2 * i + 1], h);
+                if constexpr (SPLIT) pl[b][i + 2] = other_half(pl[b][i]);
             }
         }
         st[b].low = mfma_h(a, ph[b], st[b].low);
@@ -432,40 +489,48 @@ struct Kv4TileRef {
 };
 
 // Walks the tiles of a wavefront's range, across its pieces, ahead of the
-// computation; page ids are read (scalar loads) one tile before their use.
+// computation.
 template <int D> struct Kv4Walker {
     RangeCursor cur;
     MfmaPiece pc;
     bool more;
-    int t0, blk_a, blk_b;  // the next tile: its first token and page ids
+    int t0;   // first token of the next tile
+    int ids;  // lane i: page id of cache tile first + i of the piece (past it: -1)
+    int at;   // the next tile's lane
 
-    __device__ __forceinline__ void ids(const DecodeParams &p, const int *__restrict__ tables) {
+    // Page ids of the next 64 cache tiles, in one load: one at a time they are
+    // a chain of round trips before the first tiles.
+    __device__ __forceinline__ void load_ids(const DecodeParams &p, const int *__restrict__ tables, int lane) {
         const int *bt = tables + (size_t)pc.s * p.max_blocks;
-        const int tb = t0 + kKv4Tile;
-        blk_a = bt[t0 >> p.bs_shift];
-        blk_b = tb < pc.t_end ? bt[tb >> p.bs_shift] : -1;
+        const int t = t0 + kKv4Tile * lane;
+        const int id = bt[(t < pc.t_end ? t : pc.t_end - 1) >> p.bs_shift];
+        ids = t < pc.t_end ? id : -1;
+        at = 0;
     }
     __device__ __forceinline__ void piece(const DecodeParams &p, const int *__restrict__ lens,
-                                          const int *__restrict__ tables, const int *pre) {
+                                          const int *__restrict__ tables, const int *pre, int lane) {
         more = next_piece<kKv4TileTokens>(p, lens, pre, cur, pc);
         if (more) {
             t0 = pc.t_begin;
-            ids(p, tables);
+            load_ids(p, tables, lane);
         }
     }
     __device__ __forceinline__ Kv4TileRef take(const DecodeParams &p, const int *__restrict__ lens,
-                                               const int *__restrict__ tables, const int *pre) {
+                                               const int *__restrict__ tables, const int *pre, int lane) {
         if (!more) return Kv4TileRef{0, 0, false, false};
+        const int blk_a = __builtin_amdgcn_readlane(ids, at), blk_b = __builtin_amdgcn_readlane(ids, at + 1);
         constexpr unsigned kBytes = Kv4Geometry<D>::kBytes;
         const unsigned mask = (unsigned)p.block_size - 1;
-        const long long head = (long long)pc.kvh * p.kv_head_stride;
+        // (the strides are ints at the entry: 32-bit products)
+        const long long head = (long long)pc.kvh * (int)p.kv_head_stride;
         const Kv4TileRef r = {
-            head + (long long)blk_a * p.kv_block_stride + ((((unsigned)t0 & mask) >> 4) * kBytes),
-            head + (long long)blk_b * p.kv_block_stride + ((((unsigned)t0 + 16 & mask) >> 4) * kBytes),
+            head + (long long)blk_a * (int)p.kv_block_stride + ((((unsigned)t0 & mask) >> 4) * kBytes),
+            head + (long long)blk_b * (int)p.kv_block_stride + ((((unsigned)t0 + 16 & mask) >> 4) * kBytes),
             blk_a >= 0, blk_b >= 0};
         t0 += kKv4TileTokens;
-        if (t0 < pc.t_end) ids(p, tables);
-        else piece(p, lens, tables, pre);
+        at += 2;
+        if (t0 >= pc.t_end) piece(p, lens, tables, pre, lane);
+        else if (at == 64) load_ids(p, tables, lane);
         return r;
     }
 };
@@ -480,29 +545,22 @@ __device__ __forceinline__ void kv4_fetch_half(const void *cache, const Kv4TileR
     kv4_fetch<D>((const char *)cache + r.at_b, r.b, lds + Kv4Geometry<D>::kBytes, lane);
 }
 
-// Wavefronts per SIMD the kernel is compiled for: as many as two LDS slots
-// each and the state's registers leave room for.
-constexpr int kv4_waves_per_simd(int head_size, int row_blocks) {
-    return head_size > 192 ? 1 : head_size > 128 || row_blocks > 1 ? 2 : 3;
-}
+// Wavefronts per SIMD the kernel is compiled for, and LDS slots of each.
+constexpr int kv4_waves_per_simd(int head_size) { return head_size > 192 ? 1 : 2; }
+// (A third slot measured 1-2% slower, a third wavefront spilled.)
+constexpr int kv4_slots(int) { return 2; }
 
-template <int KV, int D, int R>
-__global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D, R))) void paged_decode_partition_kv4_kernel(
-    const DecodeParams p, const int *__restrict__ lens, const int *__restrict__ tables) {
+// One wavefront's range: logical wavefront w of the plan, with its LDS slots.
+template <int KV, int D, int R, bool SPLIT>
+__device__ __forceinline__ void kv4_range(const DecodeParams &p, const int *__restrict__ lens,
+                                          const int *__restrict__ tables, const int *pre, int total, int w,
+                                          char (&slots)[kv4_slots(D)][Kv4Geometry<D>::kSlot]) {
     using G = Kv4Geometry<D>;
-    constexpr int TT = kKv4TileTokens, NG = G::NG, NF = G::kHalfFetches;
-    extern __shared__ int pre[];  // num_seqs + 1 split-unit prefixes
-    __shared__ __attribute__((aligned(16))) char slots[kKv4Waves][2][G::kSlot];
-    if (threadIdx.x < 2 * kKv4Waves)  // (the fetches leave them alone)
-        *(u32x4 *)&slots[threadIdx.x >> 1][threadIdx.x & 1][G::kOnes] =
-            u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
-    batch_prefix<TT, kKv4Waves>(p, pre);
+    constexpr int TT = kKv4TileTokens, NG = G::NG, NF = G::kHalfFetches, S = kv4_slots(D);
+    constexpr int kX = SPLIT ? 4 : 8;  // scores of a lane
+    static_assert(!SPLIT || R == 1, "split columns: one block");
     const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int total = __builtin_amdgcn_readfirstlane(pre[p.num_seqs]);
-    const int w = logical_block(p, total) * kKv4Waves + wave;
     const int tpw = tiles_per_wave(total, p.num_waves, p.min_tiles_per_wave);
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.ws_prefix[p.num_seqs + 1] = tpw;  // for the merge
     const long long g_lo = (long long)w * tpw;
     if (g_lo >= total) return;
     RangeCursor cur;
@@ -521,33 +579,40 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D, R))) void pa
     }
     Kv4Walker<D> ahead;
     ahead.cur = cur;
-    ahead.piece(p, lens, tables, pre);
+    ahead.piece(p, lens, tables, pre, lane);
     MfmaPiece pc;
     if (!next_piece<TT>(p, lens, pre, cur, pc)) return;
     // LDS address of the wavefront's slots, K half then V half of each
     const uint32_t lds0 =
-        (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)&slots[0][0][0] +
-        (uint32_t)(wave * 2 * G::kSlot);
-    Kv4TileRef at = ahead.take(p, lens, tables, pre);
-    kv4_fetch_half<D>(p.k, at, lds0, lane);
-    kv4_fetch_half<D>(p.v, at, lds0 + 2 * G::kBytes, lane);
-    Kv4TileRef then = ahead.take(p, lens, tables, pre);
-    kv4_fetch_half<D>(p.k, then, lds0 + G::kSlot, lane);
-    kv4_fetch_half<D>(p.v, then, lds0 + G::kSlot + 2 * G::kBytes, lane);
+        (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)&slots[0][0];
+    Kv4TileRef ref[S];  // the tile at hand and those behind it
+#pragma unroll
+    for (int i = 0; i < S; i++) {
+        ref[i] = ahead.take(p, lens, tables, pre, lane);
+        kv4_fetch_half<D>(p.k, ref[i], lds0 + i * G::kSlot, lane);
+        kv4_fetch_half<D>(p.v, ref[i], lds0 + i * G::kSlot + 2 * G::kBytes, lane);
+    }
     // the lane's lows of V: group j's, or past the groups the ones
     const int low_a = j < NG ? 2 * G::kBytes + kv4_v_low(NG, 4 * q, j < NG ? j : 0) : G::kOnes;
     const int low_b = j < NG ? low_a + G::kBytes : G::kOnes;
     int slot = 0;
     bool has_next = true;
+    // The wavefronts of a SIMD share it oldest first: at equal priority the
+    // younger one was left a fifth behind and finished its range alone.  A
+    // wavefront's priority falls as it gets on, so that whichever is ahead waits.
+    const int units = min(total, (int)g_lo + tpw) - (int)g_lo;
+    int left = units;  // (tiles; a segment's start-up units are left over)
+    __builtin_amdgcn_s_setprio(3);
+    XHIP_WAVE_STAMP(p, threadIdx.x >> 6, 0);
     while (has_next) {
-        Kv4Query<KV, D> qr[R];
+        Kv4Query<KV, D, SPLIT> qr[R];
         Kv4State<D> st[R];
         const int g0 = pc.ht * kMfmaHeads * R;
-        float top = kKv4Top;
+        float limit = kKv4Limit;
         uint32_t big_step = kKv4BigStep;
 #pragma unroll
         for (int b = 0; b < R; b++) {
-            kv4_load_query<KV, D>(p, pc, lane, g0 + 16 * b, p.group - g0 - 16 * b, qr[b]);
+            kv4_load_query<KV, D, SPLIT>(p, pc, lane, g0 + 16 * b, p.group - g0 - 16 * b, qr[b]);
 #pragma unroll
             for (int g = 0; g < NG; g++) st[b].o[g][0] = st[b].o[g][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             st[b].low = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -555,30 +620,51 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D, R))) void pa
             st[b].limit = -INFINITY;
         }
         for (int t0 = pc.t_begin; t0 < pc.t_end; t0 += TT) {
-            const Kv4TileRef nx = ahead.take(p, lens, tables, pre);
-            const char *ks = &slots[wave][slot][0], *vs = ks + 2 * G::kBytes;
+            left--;
+            if (left == units / 2) __builtin_amdgcn_s_setprio(2);
+            if (left == units / 4) __builtin_amdgcn_s_setprio(1);
+            if (left == units / 10) __builtin_amdgcn_s_setprio(0);
+            const Kv4TileRef nx = ahead.take(p, lens, tables, pre, lane);
+            const char *ks = &slots[slot][0], *vs = ks + 2 * G::kBytes;
             const uint32_t lds = lds0 + (uint32_t)(slot * G::kSlot);
-            float x[R][8];
-            kv4_wait<3 * NF>();  // later: this tile's V, the next one's K and V
-            kv4_scores<KV, D, R>(ks, qr, st, lane, 0, x);
-            kv4_scores<KV, D, R>(ks + G::kBytes, qr, st, lane, 4, x);
-            kv4_fetch_half<D>(p.k, nx, lds, lane);
-
-            kv4_wait<3 * NF>();  // later: the next tile's K and V, K of the one after
-            // (uniform, which the compiler cannot see)
-            if (__builtin_amdgcn_readfirstlane(t0 + TT > pc.t_end || !at.a || !at.b)) {
-                // tokens past the end or in missing pages: no weight, and no
-                // step or low of theirs (whatever the slots hold) in a product.
-                // In LDS, not in the registers: there the other way through
-                // the branch got a copy of every value.
+            float x[R][kX];
+            kv4_wait<(2 * S - 1) * NF>();  // later: this tile's V, K and V of the next S - 1
+            // tokens past the end or in missing pages (uniform, which the compiler
+            // cannot see)
+            const bool part = __builtin_amdgcn_readfirstlane(t0 + TT > pc.t_end || !ref[0].a || !ref[0].b);
+            if (SPLIT && part) {
+                // a product of b's lows with the zeros of columns 0-7 is added to
+                // a's: no NaN there, whatever the slots hold
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const int n = (h ? at.b : at.a) ? pc.t_end - t0 - 16 * h : 0;  // tokens
+                    const int n = (h ? ref[0].b : ref[0].a) ? pc.t_end - t0 - 16 * h : 0;  // tokens
+                    for (int i = lane; i < 16 * NG; i += 64)
+                        if (i / NG >= n)
+                            *(uint16_t *)(slots[slot] + h * G::kBytes + kv4_k_low(NG, i / NG, i % NG)) = 0;
+                }
+                wave_lds_fence();  // before the reads below, by other lanes
+            }
+            kv4_scores<KV, D, R, SPLIT>(ks, qr, st, lane, x);
+            kv4_fetch_half<D>(p.k, nx, lds, lane);
+
+            kv4_wait<(2 * S - 1) * NF>();  // later: K and V of the next S - 1, K of one more
+            if (part) {
+                // no weight for such a token, and no step or low of its in a
+                // product.  In LDS, not in the registers: there the other way
+                // through the branch got a copy of every value.
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
+                for (int h = 0; h < 2; h++) {
+                    const int n = (h ? ref[0].b : ref[0].a) ? pc.t_end - t0 - 16 * h : 0;  // tokens
+                    if (!SPLIT || h == 0) {
+                        // (SPLIT: the lane's scores are of the cache tile of its column)
+                        const int n_b = ref[0].b ? pc.t_end - t0 - 16 : 0;
+                        const int m = SPLIT && (lane & 8) ? n_b : n;
 #pragma unroll
-                        for (int b = 0; b < R; b++) keep_score(x[b][4 * h + e], 4 * q + e < n);
-                    uint16_t *t = (uint16_t *)(slots[wave][slot] + (2 + h) * G::kBytes);
+                        for (int e = 0; e < 4; e++)
+#pragma unroll
+                            for (int b = 0; b < R; b++) keep_score(x[b][4 * h + e], 4 * q + e < m);
+                    }
+                    uint16_t *t = (uint16_t *)(slots[slot] + (2 + h) * G::kBytes);
                     for (int i = lane; i < 16 * NG; i += 64) {
                         if ((i / (4 * NG)) * 4 + (i & 3) < n) continue;
                         t[kv4_step(NG, 0, 0) / 2 + i] = 0;
@@ -604,65 +690,104 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D, R))) void pa
                 Kv4State<D> &s = st[b];
                 float mx = x[b][0];
 #pragma unroll
-                for (int e = 1; e < 8; e++) mx = fmaxf(mx, x[b][e]);
+                for (int e = 1; e < kX; e++) mx = fmaxf(mx, x[b][e]);
                 if (big || __any(mx > s.limit)) {
-                    if (big) top = kKv4BigTop;
+                    if (big) limit = kKv4BigLimit;
+                    if constexpr (SPLIT) mx = fmaxf(mx, __shfl_xor(mx, 8));
                     mx = fmaxf(mx, __shfl_xor(mx, 16));
                     mx = fmaxf(mx, __shfl_xor(mx, 32));
                     const bool fresh = s.limit == -INFINITY;
-                    // this head's new base: where the larger of its old and
-                    // new largest scores has weight 2^top
-                    const float most = fmaxf(mx, s.limit);
-                    const bool any = most != -INFINITY;
-                    const float down = any ? most - top : 0.0f;
-                    const float alpha = fresh || down == 0.0f ? 1.0f : fast_exp2(-down);
+                    // the base moves where a score passes its limit, and where
+                    // the limit falls
+                    const bool move = mx > s.limit || (!fresh && s.limit != limit);
+                    const float most = fresh ? mx : fmaxf(mx, s.limit);
+                    const float top = limit - kKv4Slack;
+                    const float down = move ? most - top : 0.0f;
+                    const float alpha = fresh || !move ? 1.0f : fast_exp2(-down);
                     s.base += down;
-                    s.limit = any ? top : s.limit;
+                    s.limit = move ? limit : s.limit;
                     s.low *= alpha;
 #pragma unroll
                     for (int g = 0; g < NG; g++) {
                         s.o[g][0] *= alpha;
                         s.o[g][1] *= alpha;
                     }
-                    // (the largest weight is 2^top to the bit)
+                    // (the largest weight is a power of two to the bit)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[b][e] = down != 0.0f ? (x[b][e] - most) + top : x[b][e];
+                    for (int e = 0; e < kX; e++) x[b][e] = move ? (x[b][e] - most) + top : x[b][e];
                 }
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[b][e] = fast_exp2(x[b][e]);
+                for (int e = 0; e < kX; e++) x[b][e] = fast_exp2(x[b][e]);
             }
             if (big) big_step = 0;
-            kv4_pv<KV, D, R>(v, x, st);
+            kv4_pv<KV, D, R, SPLIT>(v, x, st);
             kv4_fetch_half<D>(p.v, nx, lds + 2 * G::kBytes, lane);
-            at = then;
-            then = nx;
-            slot ^= 1;
+#pragma unroll
+            for (int i = 0; i + 1 < S; i++) ref[i] = ref[i + 1];
+            ref[S - 1] = nx;
+            slot = slot + 1 == S ? 0 : slot + 1;
         }
         kv4_write<KV, D, R>(p, pc, lane, st);
         has_next = next_piece<TT>(p, lens, pre, cur, pc);
     }
+    XHIP_WAVE_STAMP(p, threadIdx.x >> 6, 1);
     kv4_wait<0>();  // nothing of this wavefront's may reach LDS after its end
+}
+
+template <int KV, int D, int R, bool SPLIT>
+__global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D))) void paged_decode_partition_kv4_kernel(
+    const DecodeParams p, const int *__restrict__ lens, const int *__restrict__ tables) {
+    using G = Kv4Geometry<D>;
+    constexpr int S = kv4_slots(D);
+    extern __shared__ int pre[];  // num_seqs + 1 split-unit prefixes
+    __shared__ __attribute__((aligned(16))) char slots[kKv4Waves][S][G::kSlot];
+    XHIP_WG_BEGIN(p);
+    if (threadIdx.x < S * kKv4Waves)  // (the fetches leave them alone)
+        *(u32x4 *)&slots[threadIdx.x / S][threadIdx.x % S][G::kOnes] =
+            u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+    batch_prefix<kKv4TileTokens, kKv4Waves>(p, pre);
+    XHIP_WG_STAMP(p, 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int total = __builtin_amdgcn_readfirstlane(pre[p.num_seqs]);
+    const int lb = logical_block(p, total);
+    XHIP_WG_PUT(p, 3, lb);
+    if (blockIdx.x == 0 && threadIdx.x == 0)  // for the merge
+        p.ws_prefix[p.num_seqs + 1] = tiles_per_wave(total, p.num_waves, p.min_tiles_per_wave);
+    kv4_range<KV, D, R, SPLIT>(p, lens, tables, pre, total, lb * kKv4Waves + wave, slots[wave]);
+    XHIP_WG_FLUSH(p);
 }
 
 // Two row blocks per wavefront for groups of 17 to 32 heads.
 constexpr bool kv4_has_wide(int head_size) { return head_size <= 128; }
 
-template <int KV, int D, int R>
-static hipError_t launch_kv4_rows_of(const DecodeParams &p, hipStream_t st, hipEvent_t ev_start,
-                                     hipEvent_t ev_stop) {
-    const hipError_t e = launch_partition(
-        paged_decode_partition_kv4_kernel<KV, D, R>, (unsigned)(p.num_waves / kKv4Waves), 64 * kKv4Waves,
-        (size_t)(p.num_seqs + 1) * sizeof(int), st, ev_start, ev_stop, p, p.seq_lens, p.block_tables);
-    if (e != hipSuccess) return e;
-    return launch_merge<KV, D, kMfmaHeads * R, kKv4TileTokens>(p, st);
+template <int KV, int D, int R, bool SPLIT>
+static hipError_t launch_kv4_kernel(const DecodeParams &p, hipStream_t st, hipEvent_t ev_start,
+                                    hipEvent_t ev_stop) {
+    return launch_partition(paged_decode_partition_kv4_kernel<KV, D, R, SPLIT>,
+                            (unsigned)(p.num_waves / kKv4Waves), 64 * kKv4Waves,
+                            (size_t)(p.num_seqs + 1) * sizeof(int), st, ev_start, ev_stop, p, p.seq_lens,
+                            p.block_tables);
 }
+
+// Groups of up to 8 heads: the columns of the score products hold them twice,
+// for a tile's two cache tiles, so that a lane has 4 scores and not 8.
+constexpr int kKv4SplitHeads = 8;
 
 template <int KV, int D>
 static hipError_t launch_kv4_size(const DecodeParams &p, int head_tile, hipStream_t st,
                                   hipEvent_t ev_start, hipEvent_t ev_stop) {
-    if constexpr (kv4_has_wide(D))
-        if (head_tile == 2 * kMfmaHeads) return launch_kv4_rows_of<KV, D, 2>(p, st, ev_start, ev_stop);
-    return launch_kv4_rows_of<KV, D, 1>(p, st, ev_start, ev_stop);
+    if constexpr (kv4_has_wide(D)) {
+        if (head_tile == 2 * kMfmaHeads) {
+            const hipError_t e = launch_kv4_kernel<KV, D, 2, false>(p, st, ev_start, ev_stop);
+            if (e != hipSuccess) return e;
+            return launch_merge<KV, D, 2 * kMfmaHeads, kKv4TileTokens>(p, st);
+        }
+    }
+    const hipError_t e = p.group <= kKv4SplitHeads
+                             ? launch_kv4_kernel<KV, D, 1, true>(p, st, ev_start, ev_stop)
+                             : launch_kv4_kernel<KV, D, 1, false>(p, st, ev_start, ev_stop);
+    if (e != hipSuccess) return e;
+    return launch_merge<KV, D, kMfmaHeads, kKv4TileTokens>(p, st);
 }
 
 template <int KV>
@@ -677,18 +802,20 @@ static hipError_t launch_kv4_dtype(const DecodeParams &p, int head_size, int hea
     }
 }
 
-template <int KV, int D> static const void *kv4_fn(int head_tile) {
+template <int KV, int D> static const void *kv4_fn(int head_tile, int group) {
     if constexpr (kv4_has_wide(D))
         if (head_tile == 2 * kMfmaHeads)
-            return reinterpret_cast<const void *>(&paged_decode_partition_kv4_kernel<KV, D, 2>);
-    return reinterpret_cast<const void *>(&paged_decode_partition_kv4_kernel<KV, D, 1>);
+            return reinterpret_cast<const void *>(&paged_decode_partition_kv4_kernel<KV, D, 2, false>);
+    return group <= kKv4SplitHeads
+               ? reinterpret_cast<const void *>(&paged_decode_partition_kv4_kernel<KV, D, 1, true>)
+               : reinterpret_cast<const void *>(&paged_decode_partition_kv4_kernel<KV, D, 1, false>);
 }
 
-template <int KV> static int kv4_occupancy_dtype(int head_size, int head_tile, size_t lds_bytes) {
+template <int KV> static int kv4_occupancy_dtype(int head_size, int head_tile, int group, size_t lds_bytes) {
     const void *fn = nullptr;
     switch (head_size) {
 #define XHIP_CASE(d) \
-    case d: fn = kv4_fn<KV, d>(head_tile); break;
+    case d: fn = kv4_fn<KV, d>(head_tile, group); break;
         XHIP_FOR_HEAD_SIZES(XHIP_CASE)
 #undef XHIP_CASE
     default: return 0;

@@ -3,8 +3,8 @@
 
 namespace xhip {
 
-int kv4_occupancy_bf16(int head_size, int head_tile, size_t lds_bytes) {
-    return kv4_occupancy_dtype<KV_BF16>(head_size, head_tile, lds_bytes);
+int kv4_occupancy_bf16(int head_size, int head_tile, int group, size_t lds_bytes) {
+    return kv4_occupancy_dtype<KV_BF16>(head_size, head_tile, group, lds_bytes);
 }
 
 hipError_t launch_kv4_bf16(const DecodeParams &p, int head_size, int head_tile, hipStream_t stream,

@@ -33,9 +33,9 @@ hipError_t launch_decode_f32(const DecodeParams &p, int head_size, int head_tile
 // The decode attention over a 4-bit K/V cache (paged_decode_kv4.h), by the
 // dtype of query and output: resident workgroups (of kMfmaWavesPerGroup
 // wavefronts) per CU, and the two launches.
-int kv4_occupancy_f16(int head_size, int head_tile, size_t lds_bytes);
-int kv4_occupancy_bf16(int head_size, int head_tile, size_t lds_bytes);
-int kv4_occupancy_f32(int head_size, int head_tile, size_t lds_bytes);
+int kv4_occupancy_f16(int head_size, int head_tile, int group, size_t lds_bytes);
+int kv4_occupancy_bf16(int head_size, int head_tile, int group, size_t lds_bytes);
+int kv4_occupancy_f32(int head_size, int head_tile, int group, size_t lds_bytes);
 hipError_t launch_kv4_f16(const DecodeParams &p, int head_size, int head_tile, hipStream_t stream,
                           hipEvent_t ev_start, hipEvent_t ev_stop);
 hipError_t launch_kv4_bf16(const DecodeParams &p, int head_size, int head_tile, hipStream_t stream,
