@@ -489,36 +489,36 @@ struct Kv4TileRef {
 };
 
 // Walks the tiles of a wavefront's range, across its pieces, ahead of the
-// computation.
+// computation.  Page ids are scalar loads, two tiles ahead: as vector loads they
+// would be waited for behind every fetch in flight.
 template <int D> struct Kv4Walker {
     RangeCursor cur;
     MfmaPiece pc;
     bool more;
-    int t0;   // first token of the next tile
-    int ids;  // lane i: page id of cache tile first + i of the piece (past it: -1)
-    int at;   // the next tile's lane
+    int t0;                  // first token of the next tile
+    int blk[2], blk_then[2];  // page ids of its cache tiles, and of the tile behind it
 
-    // Page ids of the next 64 cache tiles, in one load: one at a time they are
-    // a chain of round trips before the first tiles.
-    __device__ __forceinline__ void load_ids(const DecodeParams &p, const int *__restrict__ tables, int lane) {
+    // Page id of the cache tile at token t of the piece (past its end: -1).
+    __device__ __forceinline__ int id(const DecodeParams &p, const int *__restrict__ tables, int t) const {
         const int *bt = tables + (size_t)pc.s * p.max_blocks;
-        const int t = t0 + kKv4Tile * lane;
-        const int id = bt[(t < pc.t_end ? t : pc.t_end - 1) >> p.bs_shift];
-        ids = t < pc.t_end ? id : -1;
-        at = 0;
+        const int b = bt[(t < pc.t_end ? t : pc.t_end - 1) >> p.bs_shift];
+        return t < pc.t_end ? b : -1;
     }
     __device__ __forceinline__ void piece(const DecodeParams &p, const int *__restrict__ lens,
-                                          const int *__restrict__ tables, const int *pre, int lane) {
+                                          const int *__restrict__ tables, const int *pre) {
         more = next_piece<kKv4TileTokens>(p, lens, pre, cur, pc);
         if (more) {
             t0 = pc.t_begin;
-            load_ids(p, tables, lane);
+            for (int i = 0; i < 2; i++) {
+                blk[i] = id(p, tables, t0 + kKv4Tile * i);
+                blk_then[i] = id(p, tables, t0 + kKv4Tile * (2 + i));
+            }
         }
     }
     __device__ __forceinline__ Kv4TileRef take(const DecodeParams &p, const int *__restrict__ lens,
-                                               const int *__restrict__ tables, const int *pre, int lane) {
+                                               const int *__restrict__ tables, const int *pre) {
         if (!more) return Kv4TileRef{0, 0, false, false};
-        const int blk_a = __builtin_amdgcn_readlane(ids, at), blk_b = __builtin_amdgcn_readlane(ids, at + 1);
+        const int blk_a = blk[0], blk_b = blk[1];
         constexpr unsigned kBytes = Kv4Geometry<D>::kBytes;
         const unsigned mask = (unsigned)p.block_size - 1;
         // (the strides are ints at the entry: 32-bit products)
@@ -528,9 +528,14 @@ template <int D> struct Kv4Walker {
             head + (long long)blk_b * (int)p.kv_block_stride + ((((unsigned)t0 + 16 & mask) >> 4) * kBytes),
             blk_a >= 0, blk_b >= 0};
         t0 += kKv4TileTokens;
-        at += 2;
-        if (t0 >= pc.t_end) piece(p, lens, tables, pre, lane);
-        else if (at == 64) load_ids(p, tables, lane);
+        if (t0 >= pc.t_end) {
+            piece(p, lens, tables, pre);
+        } else {
+            for (int i = 0; i < 2; i++) {
+                blk[i] = blk_then[i];
+                blk_then[i] = id(p, tables, t0 + kKv4Tile * (2 + i));
+            }
+        }
         return r;
     }
 };
@@ -548,28 +553,43 @@ __device__ __forceinline__ void kv4_fetch_half(const void *cache, const Kv4TileR
 // Wavefronts per SIMD the kernel is compiled for, and LDS slots of each.
 constexpr int kv4_waves_per_simd(int head_size) { return head_size > 192 ? 1 : 2; }
 // (A third slot measured 1-2% slower, a third wavefront spilled.)
-constexpr int kv4_slots(int) { return 2; }
+constexpr int kKv4Slots = 2;
 
-// One wavefront's range: logical wavefront w of the plan, with its LDS slots.
+// A wavefront computes one range of the plan.  (All of it stands in the kernel
+// itself: the lengths and page ids are scalar loads only where the compiler sees
+// that they come from the kernel's own restrict arguments.)
 template <int KV, int D, int R, bool SPLIT>
-__device__ __forceinline__ void kv4_range(const DecodeParams &p, const int *__restrict__ lens,
-                                          const int *__restrict__ tables, const int *pre, int total, int w,
-                                          char (&slots)[kv4_slots(D)][Kv4Geometry<D>::kSlot]) {
+__global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D))) void paged_decode_partition_kv4_kernel(
+    const DecodeParams p, const int *__restrict__ lens, const int *__restrict__ tables) {
     using G = Kv4Geometry<D>;
-    constexpr int TT = kKv4TileTokens, NG = G::NG, NF = G::kHalfFetches, S = kv4_slots(D);
+    constexpr int TT = kKv4TileTokens, NG = G::NG, NF = G::kHalfFetches, S = kKv4Slots;
     constexpr int kX = SPLIT ? 4 : 8;  // scores of a lane
     static_assert(!SPLIT || R == 1, "split columns: one block");
+    extern __shared__ int pre[];  // num_seqs + 1 split-unit prefixes
+    __shared__ __attribute__((aligned(16))) char slots[kKv4Waves][S][G::kSlot];
+    XHIP_WG_BEGIN(p);
+    if (threadIdx.x < S * kKv4Waves)  // (the fetches leave them alone)
+        *(u32x4 *)&slots[threadIdx.x / S][threadIdx.x % S][G::kOnes] =
+            u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+    batch_prefix<TT, kKv4Waves>(p, pre);
+    XHIP_WG_STAMP(p, 1);
     const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int total = __builtin_amdgcn_readfirstlane(pre[p.num_seqs]);
+    const int lb = logical_block(p, total);
+    XHIP_WG_PUT(p, 3, lb);
+    const int w = lb * kKv4Waves + wave;
     const int tpw = tiles_per_wave(total, p.num_waves, p.min_tiles_per_wave);
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.ws_prefix[p.num_seqs + 1] = tpw;  // for the merge
     const long long g_lo = (long long)w * tpw;
-    if (g_lo >= total) return;
     RangeCursor cur;
     cur.g = (int)g_lo;
-    cur.g_end = min(total, cur.g + tpw);
+    cur.g_end = g_lo < total ? min(total, cur.g + tpw) : cur.g;
     cur.first = 1;
     cur.w = w;
     cur.ht = -1;
-    {
+    cur.s = 0;
+    if (g_lo < total) {
         int lo = 0, hi = p.num_seqs - 1;  // the sequence holding unit g
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -577,183 +597,153 @@ __device__ __forceinline__ void kv4_range(const DecodeParams &p, const int *__re
         }
         cur.s = __builtin_amdgcn_readfirstlane(lo);
     }
-    Kv4Walker<D> ahead;
-    ahead.cur = cur;
-    ahead.piece(p, lens, tables, pre, lane);
+    const RangeCursor start = cur;
     MfmaPiece pc;
-    if (!next_piece<TT>(p, lens, pre, cur, pc)) return;
-    // LDS address of the wavefront's slots, K half then V half of each
-    const uint32_t lds0 =
-        (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)&slots[0][0];
-    Kv4TileRef ref[S];  // the tile at hand and those behind it
+    bool has_next = next_piece<TT>(p, lens, pre, cur, pc);
+    if (has_next) {
+        Kv4Walker<D> ahead;
+        ahead.cur = start;
+        ahead.piece(p, lens, tables, pre);
+        // LDS address of the wavefront's slots, K half then V half of each
+        const uint32_t lds0 =
+            (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)&slots[wave][0][0];
+        Kv4TileRef ref[S];  // the tile at hand and those behind it
 #pragma unroll
-    for (int i = 0; i < S; i++) {
-        ref[i] = ahead.take(p, lens, tables, pre, lane);
-        kv4_fetch_half<D>(p.k, ref[i], lds0 + i * G::kSlot, lane);
-        kv4_fetch_half<D>(p.v, ref[i], lds0 + i * G::kSlot + 2 * G::kBytes, lane);
-    }
-    // the lane's lows of V: group j's, or past the groups the ones
-    const int low_a = j < NG ? 2 * G::kBytes + kv4_v_low(NG, 4 * q, j < NG ? j : 0) : G::kOnes;
-    const int low_b = j < NG ? low_a + G::kBytes : G::kOnes;
-    int slot = 0;
-    bool has_next = true;
-    // The wavefronts of a SIMD share it oldest first: at equal priority the
-    // younger one was left a fifth behind and finished its range alone.  A
-    // wavefront's priority falls as it gets on, so that whichever is ahead waits.
-    const int units = min(total, (int)g_lo + tpw) - (int)g_lo;
-    int left = units;  // (tiles; a segment's start-up units are left over)
-    __builtin_amdgcn_s_setprio(3);
-    XHIP_WAVE_STAMP(p, threadIdx.x >> 6, 0);
-    while (has_next) {
-        Kv4Query<KV, D, SPLIT> qr[R];
-        Kv4State<D> st[R];
-        const int g0 = pc.ht * kMfmaHeads * R;
-        float limit = kKv4Limit;
-        uint32_t big_step = kKv4BigStep;
-#pragma unroll
-        for (int b = 0; b < R; b++) {
-            kv4_load_query<KV, D, SPLIT>(p, pc, lane, g0 + 16 * b, p.group - g0 - 16 * b, qr[b]);
-#pragma unroll
-            for (int g = 0; g < NG; g++) st[b].o[g][0] = st[b].o[g][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            st[b].low = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            st[b].base = 0.0f;
-            st[b].limit = -INFINITY;
+        for (int i = 0; i < S; i++) {
+            ref[i] = ahead.take(p, lens, tables, pre);
+            kv4_fetch_half<D>(p.k, ref[i], lds0 + i * G::kSlot, lane);
+            kv4_fetch_half<D>(p.v, ref[i], lds0 + i * G::kSlot + 2 * G::kBytes, lane);
         }
-        for (int t0 = pc.t_begin; t0 < pc.t_end; t0 += TT) {
-            left--;
-            if (left == units / 2) __builtin_amdgcn_s_setprio(2);
-            if (left == units / 4) __builtin_amdgcn_s_setprio(1);
-            if (left == units / 10) __builtin_amdgcn_s_setprio(0);
-            const Kv4TileRef nx = ahead.take(p, lens, tables, pre, lane);
-            const char *ks = &slots[slot][0], *vs = ks + 2 * G::kBytes;
-            const uint32_t lds = lds0 + (uint32_t)(slot * G::kSlot);
-            float x[R][kX];
-            kv4_wait<(2 * S - 1) * NF>();  // later: this tile's V, K and V of the next S - 1
-            // tokens past the end or in missing pages (uniform, which the compiler
-            // cannot see)
-            const bool part = __builtin_amdgcn_readfirstlane(t0 + TT > pc.t_end || !ref[0].a || !ref[0].b);
-            if (SPLIT && part) {
-                // a product of b's lows with the zeros of columns 0-7 is added to
-                // a's: no NaN there, whatever the slots hold
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int n = (h ? ref[0].b : ref[0].a) ? pc.t_end - t0 - 16 * h : 0;  // tokens
-                    for (int i = lane; i < 16 * NG; i += 64)
-                        if (i / NG >= n)
-                            *(uint16_t *)(slots[slot] + h * G::kBytes + kv4_k_low(NG, i / NG, i % NG)) = 0;
-                }
-                wave_lds_fence();  // before the reads below, by other lanes
-            }
-            kv4_scores<KV, D, R, SPLIT>(ks, qr, st, lane, x);
-            kv4_fetch_half<D>(p.k, nx, lds, lane);
-
-            kv4_wait<(2 * S - 1) * NF>();  // later: K and V of the next S - 1, K of one more
-            if (part) {
-                // no weight for such a token, and no step or low of its in a
-                // product.  In LDS, not in the registers: there the other way
-                // through the branch got a copy of every value.
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int n = (h ? ref[0].b : ref[0].a) ? pc.t_end - t0 - 16 * h : 0;  // tokens
-                    if (!SPLIT || h == 0) {
-                        // (SPLIT: the lane's scores are of the cache tile of its column)
-                        const int n_b = ref[0].b ? pc.t_end - t0 - 16 : 0;
-                        const int m = SPLIT && (lane & 8) ? n_b : n;
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-#pragma unroll
-                            for (int b = 0; b < R; b++) keep_score(x[b][4 * h + e], 4 * q + e < m);
-                    }
-                    uint16_t *t = (uint16_t *)(slots[slot] + (2 + h) * G::kBytes);
-                    for (int i = lane; i < 16 * NG; i += 64) {
-                        if ((i / (4 * NG)) * 4 + (i & 3) < n) continue;
-                        t[kv4_step(NG, 0, 0) / 2 + i] = 0;
-                        t[kv4_v_low(NG, 0, 0) / 2 + i] = 0;
-                    }
-                }
-                wave_lds_fence();  // before the reads below, by other lanes
-            }
-            Kv4Values<D> v;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const char *t = vs + h * G::kBytes;
-                lds_words(t + kv4_v_word(NG, q, j, 0), v.code[h]);
-                lds_words(t + kv4_step(NG, 4 * q, 0), v.step[h]);
-                lds_words(ks + (h ? low_b : low_a), v.low[h]);
-            }
-            uint32_t steps = 0;
-#pragma unroll
-            for (int g = 0; g < 2 * NG; g++) steps |= v.step[0][g] | v.step[1][g];
-            const bool big = __any((steps & big_step) != 0);
+        // the lane's lows of V: group j's, or past the groups the ones
+        const int low_a = j < NG ? 2 * G::kBytes + kv4_v_low(NG, 4 * q, j < NG ? j : 0) : G::kOnes;
+        const int low_b = j < NG ? low_a + G::kBytes : G::kOnes;
+        int slot = 0;
+        if (threadIdx.x < 64 * kMfmaWavesPerGroup) XHIP_WAVE_STAMP(p, threadIdx.x >> 6, 0);  // (a record holds four)
+        while (has_next) {
+            Kv4Query<KV, D, SPLIT> qr[R];
+            Kv4State<D> st[R];
+            const int g0 = pc.ht * kMfmaHeads * R;
+            float limit = kKv4Limit;
+            uint32_t big_step = kKv4BigStep;
 #pragma unroll
             for (int b = 0; b < R; b++) {
-                Kv4State<D> &s = st[b];
-                float mx = x[b][0];
+                kv4_load_query<KV, D, SPLIT>(p, pc, lane, g0 + 16 * b, p.group - g0 - 16 * b, qr[b]);
 #pragma unroll
-                for (int e = 1; e < kX; e++) mx = fmaxf(mx, x[b][e]);
-                if (big || __any(mx > s.limit)) {
-                    if (big) limit = kKv4BigLimit;
-                    if constexpr (SPLIT) mx = fmaxf(mx, __shfl_xor(mx, 8));
-                    mx = fmaxf(mx, __shfl_xor(mx, 16));
-                    mx = fmaxf(mx, __shfl_xor(mx, 32));
-                    const bool fresh = s.limit == -INFINITY;
-                    // the base moves where a score passes its limit, and where
-                    // the limit falls
-                    const bool move = mx > s.limit || (!fresh && s.limit != limit);
-                    const float most = fresh ? mx : fmaxf(mx, s.limit);
-                    const float top = limit - kKv4Slack;
-                    const float down = move ? most - top : 0.0f;
-                    const float alpha = fresh || !move ? 1.0f : fast_exp2(-down);
-                    s.base += down;
-                    s.limit = move ? limit : s.limit;
-                    s.low *= alpha;
-#pragma unroll
-                    for (int g = 0; g < NG; g++) {
-                        s.o[g][0] *= alpha;
-                        s.o[g][1] *= alpha;
-                    }
-                    // (the largest weight is a power of two to the bit)
-#pragma unroll
-                    for (int e = 0; e < kX; e++) x[b][e] = move ? (x[b][e] - most) + top : x[b][e];
-                }
-#pragma unroll
-                for (int e = 0; e < kX; e++) x[b][e] = fast_exp2(x[b][e]);
+                for (int g = 0; g < NG; g++) st[b].o[g][0] = st[b].o[g][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                st[b].low = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                st[b].base = 0.0f;
+                st[b].limit = -INFINITY;
             }
-            if (big) big_step = 0;
-            kv4_pv<KV, D, R, SPLIT>(v, x, st);
-            kv4_fetch_half<D>(p.v, nx, lds + 2 * G::kBytes, lane);
+            for (int t0 = pc.t_begin; t0 < pc.t_end; t0 += TT) {
+                const Kv4TileRef nx = ahead.take(p, lens, tables, pre);
+                const char *ks = &slots[wave][slot][0], *vs = ks + 2 * G::kBytes;
+                const uint32_t lds = lds0 + (uint32_t)(slot * G::kSlot);
+                float x[R][kX];
+                kv4_wait<(2 * S - 1) * NF>();  // later: this tile's V, K and V of the next S - 1
+                // tokens past the end or in missing pages (uniform, which the compiler
+                // cannot see)
+                const bool part = __builtin_amdgcn_readfirstlane(t0 + TT > pc.t_end || !ref[0].a || !ref[0].b);
+                if (SPLIT && part) {
+                    // a product of b's lows with the zeros of columns 0-7 is added to
+                    // a's: no NaN there, whatever the slots hold
 #pragma unroll
-            for (int i = 0; i + 1 < S; i++) ref[i] = ref[i + 1];
-            ref[S - 1] = nx;
-            slot = slot + 1 == S ? 0 : slot + 1;
-        }
-        kv4_write<KV, D, R>(p, pc, lane, st);
-        has_next = next_piece<TT>(p, lens, pre, cur, pc);
-    }
-    XHIP_WAVE_STAMP(p, threadIdx.x >> 6, 1);
-    kv4_wait<0>();  // nothing of this wavefront's may reach LDS after its end
-}
+                    for (int h = 0; h < 2; h++) {
+                        const int n = (h ? ref[0].b : ref[0].a) ? pc.t_end - t0 - 16 * h : 0;  // tokens
+                        for (int i = lane; i < 16 * NG; i += 64)
+                            if (i / NG >= n)
+                                *(uint16_t *)(slots[wave][slot] + h * G::kBytes + kv4_k_low(NG, i / NG, i % NG)) = 0;
+                    }
+                    wave_lds_fence();  // before the reads below, by other lanes
+                }
+                kv4_scores<KV, D, R, SPLIT>(ks, qr, st, lane, x);
+                kv4_fetch_half<D>(p.k, nx, lds, lane);
 
-template <int KV, int D, int R, bool SPLIT>
-__global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D))) void paged_decode_partition_kv4_kernel(
-    const DecodeParams p, const int *__restrict__ lens, const int *__restrict__ tables) {
-    using G = Kv4Geometry<D>;
-    constexpr int S = kv4_slots(D);
-    extern __shared__ int pre[];  // num_seqs + 1 split-unit prefixes
-    __shared__ __attribute__((aligned(16))) char slots[kKv4Waves][S][G::kSlot];
-    XHIP_WG_BEGIN(p);
-    if (threadIdx.x < S * kKv4Waves)  // (the fetches leave them alone)
-        *(u32x4 *)&slots[threadIdx.x / S][threadIdx.x % S][G::kOnes] =
-            u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
-    batch_prefix<kKv4TileTokens, kKv4Waves>(p, pre);
-    XHIP_WG_STAMP(p, 1);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int total = __builtin_amdgcn_readfirstlane(pre[p.num_seqs]);
-    const int lb = logical_block(p, total);
-    XHIP_WG_PUT(p, 3, lb);
-    if (blockIdx.x == 0 && threadIdx.x == 0)  // for the merge
-        p.ws_prefix[p.num_seqs + 1] = tiles_per_wave(total, p.num_waves, p.min_tiles_per_wave);
-    kv4_range<KV, D, R, SPLIT>(p, lens, tables, pre, total, lb * kKv4Waves + wave, slots[wave]);
+                kv4_wait<(2 * S - 1) * NF>();  // later: K and V of the next S - 1, K of one more
+                if (part) {
+                    // no weight for such a token, and no step or low of its in a
+                    // product.  In LDS, not in the registers: there the other way
+                    // through the branch got a copy of every value.
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int n = (h ? ref[0].b : ref[0].a) ? pc.t_end - t0 - 16 * h : 0;  // tokens
+                        if (!SPLIT || h == 0) {
+                            // (SPLIT: the lane's scores are of the cache tile of its column)
+                            const int n_b = ref[0].b ? pc.t_end - t0 - 16 : 0;
+                            const int m = SPLIT && (lane & 8) ? n_b : n;
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+#pragma unroll
+                                for (int b = 0; b < R; b++) keep_score(x[b][4 * h + e], 4 * q + e < m);
+                        }
+                        uint16_t *t = (uint16_t *)(slots[wave][slot] + (2 + h) * G::kBytes);
+                        for (int i = lane; i < 16 * NG; i += 64) {
+                            if ((i / (4 * NG)) * 4 + (i & 3) < n) continue;
+                            t[kv4_step(NG, 0, 0) / 2 + i] = 0;
+                            t[kv4_v_low(NG, 0, 0) / 2 + i] = 0;
+                        }
+                    }
+                    wave_lds_fence();  // before the reads below, by other lanes
+                }
+                Kv4Values<D> v;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const char *t = vs + h * G::kBytes;
+                    lds_words(t + kv4_v_word(NG, q, j, 0), v.code[h]);
+                    lds_words(t + kv4_step(NG, 4 * q, 0), v.step[h]);
+                    lds_words(ks + (h ? low_b : low_a), v.low[h]);
+                }
+                uint32_t steps = 0;
+#pragma unroll
+                for (int g = 0; g < 2 * NG; g++) steps |= v.step[0][g] | v.step[1][g];
+                const bool big = __any((steps & big_step) != 0);
+#pragma unroll
+                for (int b = 0; b < R; b++) {
+                    Kv4State<D> &s = st[b];
+                    float mx = x[b][0];
+#pragma unroll
+                    for (int e = 1; e < kX; e++) mx = fmaxf(mx, x[b][e]);
+                    if (big || __any(mx > s.limit)) {
+                        if (big) limit = kKv4BigLimit;
+                        if constexpr (SPLIT) mx = fmaxf(mx, __shfl_xor(mx, 8));
+                        mx = fmaxf(mx, __shfl_xor(mx, 16));
+                        mx = fmaxf(mx, __shfl_xor(mx, 32));
+                        const bool fresh = s.limit == -INFINITY;
+                        // the base moves where a score passes its limit, and where
+                        // the limit falls
+                        const bool move = mx > s.limit || (!fresh && s.limit != limit);
+                        const float most = fresh ? mx : fmaxf(mx, s.limit);
+                        const float top = limit - kKv4Slack;
+                        const float down = move ? most - top : 0.0f;
+                        const float alpha = fresh || !move ? 1.0f : fast_exp2(-down);
+                        s.base += down;
+                        s.limit = move ? limit : s.limit;
+                        s.low *= alpha;
+#pragma unroll
+                        for (int g = 0; g < NG; g++) {
+                            s.o[g][0] *= alpha;
+                            s.o[g][1] *= alpha;
+                        }
+                        // (the largest weight is a power of two to the bit)
+#pragma unroll
+                        for (int e = 0; e < kX; e++) x[b][e] = move ? (x[b][e] - most) + top : x[b][e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < kX; e++) x[b][e] = fast_exp2(x[b][e]);
+                }
+                if (big) big_step = 0;
+                kv4_pv<KV, D, R, SPLIT>(v, x, st);
+                kv4_fetch_half<D>(p.v, nx, lds + 2 * G::kBytes, lane);
+#pragma unroll
+                for (int i = 0; i + 1 < S; i++) ref[i] = ref[i + 1];
+                ref[S - 1] = nx;
+                slot = slot + 1 == S ? 0 : slot + 1;
+            }
+            kv4_write<KV, D, R>(p, pc, lane, st);
+            has_next = next_piece<TT>(p, lens, pre, cur, pc);
+        }
+        if (threadIdx.x < 64 * kMfmaWavesPerGroup) XHIP_WAVE_STAMP(p, threadIdx.x >> 6, 1);
+        kv4_wait<0>();  // nothing of this wavefront's may reach LDS after its end
+    }
     XHIP_WG_FLUSH(p);
 }
 
