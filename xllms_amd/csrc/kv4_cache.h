@@ -31,7 +31,7 @@ struct Kv4RowParams {
     int max_ctx;               // max_blocks * block_size
     // set by launch_kv4_rows for each of its launches:
     int tok0;                  // first token of the launch
-    uint32_t lanes;            // 8-channel pieces of K (and of V) rows in the launch
+    uint32_t items;            // 8-channel pieces of K (and of V) rows of 4 tokens each
     DivMagic row_div;          // division by the pieces of a row
     DivMagic head_div;         // division by num_kv_heads
 };
