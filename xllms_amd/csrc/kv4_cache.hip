@@ -10,7 +10,12 @@
 // quad of slots, as a prompt's do, each lane exchanges bytes with the other
 // tokens' lanes and moves one whole word; else it moves 4 bytes.  (A lane per
 // piece and 4 bytes each moved 32768 tokens of 8 kv heads of 128 channels, bf16,
-// 176 MB, in 59 us to the cache and 41 us out of it.)
+// 176 MB, in 59 us to the cache and 41 us out of it; this takes 47 and 33.)
+// Memory bounds it: 49152 tokens of 8 kv heads of 256 channels, fp16, out of
+// the cache, 529 MB, take 127 us, 4.2 TB/s (a large copy reaches 5.1); the
+// 16-bit rows go past the caches (137 us with ordinary stores).  Blocks of two
+// wavefronts write 32768 tokens' rows 2 us sooner than blocks of four, and read
+// as fast.
 // In fp32, and part of the format (a reader of the header can repeat it to the
 // bit):
 //   x' = x clamped to +-65504
@@ -27,7 +32,7 @@
 
 namespace xhip {
 
-constexpr int kKv4RowBlock = 256;
+constexpr int kKv4RowBlock = 128;
 constexpr long long kKv4MaxItems = (1LL << 29) - 1;  // four lanes each, a launch's lanes below 2^31
 
 // 8 elements of a row piece, as fp32.
@@ -48,7 +53,7 @@ template <int KV> __device__ __forceinline__ void store_piece(void *rows, size_t
         *(f32x4 *)dst = f32x4{x[0], x[1], x[2], x[3]};
         *(f32x4 *)(dst + 4) = f32x4{x[4], x[5], x[6], x[7]};
     } else {
-        *(u32x4 *)((char *)rows + i * 2) = float_to_chunk<KV, 8>(x);
+        __builtin_nontemporal_store((float_to_chunk<KV, 8>(x)), (u32x4 *)((char *)rows + i * 2));
     }
 }
 
@@ -159,9 +164,11 @@ __global__ __launch_bounds__(kKv4RowBlock) void kv4_rows_kernel(const Kv4RowPara
     const int vw = kv4_v_word(ng, t >> 2, 4 * q + k, g);
     const int vb = kv4_v_word(ng, t >> 2, 4 * q, g) + kv4_v_byte(t & 3);
     const int vpair = 4 * ng;  // bytes from one channel pair's word to the next
-    const int at_step = kv4_step(ng, t, g), k_low = kv4_k_low(ng, t, g), v_low = kv4_v_low(ng, t, g);
+    // the quad's lanes store one parameter of the group each: K step, K low, V step, V low
+    const int param = q == 1 ? kv4_k_low(ng, t, g) : q == 3 ? kv4_v_low(ng, t, g) : kv4_step(ng, t, g);
     const size_t elem = ((size_t)tok * p.num_kv_heads + h) * p.head_size + (size_t)c * 8;
     char *kt = p.key_cache + base, *vt = p.value_cache + base;
+    uint16_t *pt = (uint16_t *)((q < 2 ? kt : vt) + param);
     if constexpr (OP == KV4_WRITE) {
         // (lanes of skipped tokens go along, with nothing read or written: their
         // neighbours exchange with them)
@@ -190,12 +197,7 @@ __global__ __launch_bounds__(kKv4RowBlock) void kv4_rows_kernel(const Kv4RowPara
 #pragma unroll
             for (int e = 0; e < 4; e++) *(uint8_t *)(vt + vb + e * vpair) = (uint8_t)(v >> (8 * e));
         }
-        if (q == 0) {
-            *(uint16_t *)(kt + at_step) = a.step;
-            *(uint16_t *)(kt + k_low) = a.low;
-            *(uint16_t *)(vt + at_step) = b.step;
-            *(uint16_t *)(vt + v_low) = b.low;
-        }
+        *pt = q == 0 ? a.step : q == 1 ? a.low : q == 2 ? b.step : b.low;
     } else if constexpr (OP == KV4_READ) {
         uint32_t w = 0, v = 0, word = 0;
         float ks = 0.0f, kl = 0.0f, vs = 0.0f, vl = 0.0f;
@@ -207,10 +209,12 @@ __global__ __launch_bounds__(kKv4RowBlock) void kv4_rows_kernel(const Kv4RowPara
 #pragma unroll
                 for (int e = 0; e < 4; e++) v |= (uint32_t)*(const uint8_t *)(vt + vb + e * vpair) << (8 * e);
             }
-            ks = half_bits(*(const uint16_t *)(kt + at_step));
-            kl = half_bits(*(const uint16_t *)(kt + k_low));
-            vs = half_bits(*(const uint16_t *)(vt + at_step));
-            vl = half_bits(*(const uint16_t *)(vt + v_low));
+            // (one load each: a load per lane and four quad_perms were 8% slower
+            // on rows of 256 channels)
+            ks = half_bits(*(const uint16_t *)(kt + kv4_step(ng, t, g)));
+            kl = half_bits(*(const uint16_t *)(kt + kv4_k_low(ng, t, g)));
+            vs = half_bits(*(const uint16_t *)(vt + kv4_step(ng, t, g)));
+            vl = half_bits(*(const uint16_t *)(vt + kv4_v_low(ng, t, g)));
         }
         const uint32_t mine = swap_bytes(word, lane, false);
         if (whole) v = mine;
@@ -236,12 +240,8 @@ __global__ __launch_bounds__(kKv4RowBlock) void kv4_rows_kernel(const Kv4RowPara
 #pragma unroll
         for (int e = 0; e < 4; e++)
             *(uint8_t *)(vt + vb + e * vpair) = *(const uint8_t *)(vs + ub + e * vpair);
-        if (q == 0) {
-            *(uint16_t *)(kt + at_step) = *(const uint16_t *)(ks + kv4_step(ng, u, g));
-            *(uint16_t *)(kt + k_low) = *(const uint16_t *)(ks + kv4_k_low(ng, u, g));
-            *(uint16_t *)(vt + at_step) = *(const uint16_t *)(vs + kv4_step(ng, u, g));
-            *(uint16_t *)(vt + v_low) = *(const uint16_t *)(vs + kv4_v_low(ng, u, g));
-        }
+        const int from_param = q == 1 ? kv4_k_low(ng, u, g) : q == 3 ? kv4_v_low(ng, u, g) : kv4_step(ng, u, g);
+        *pt = *(const uint16_t *)((q < 2 ? ks : vs) + from_param);
     }
 }
 
