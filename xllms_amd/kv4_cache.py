@@ -19,14 +19,26 @@ arithmetic).
 """
 from __future__ import annotations
 
-import ctypes
-
 from . import _lib
-from .paged_attention import (NXT_ATTN_OK, PagedAttentionError, _ptr, _stream_handle,
-                              kv_dtype_of)
+from .paged_attention import NXT_ATTN_OK, PagedAttentionError, _stream_handle, kv_dtype_of
 
 GROUP = 32  # channels that share a range
 TILE = 16   # tokens of a tile: the smallest block_size
+
+_int32 = _uint8 = _device_of = None  # of torch, which is imported on first use
+
+
+def _current_device() -> int:
+    """Index of the current GPU (-2 before torch has initialised one, which no
+    tensor's get_device() is).  The checks here are what a small call's time
+    goes into: plain attribute reads, no Device objects."""
+    global _int32, _uint8, _device_of
+    if _device_of is None:
+        import torch
+        if not torch.cuda.is_initialized():
+            return -2
+        _int32, _uint8, _device_of = torch.int32, torch.uint8, torch.cuda.current_device
+    return _device_of()
 
 
 def _page_bytes(head_size: int, block_size: int) -> int:
@@ -57,50 +69,49 @@ def kv4_cache_empty(num_blocks: int, num_kv_heads: int, head_size: int, block_si
                        dtype=torch.uint8, device=device)
 
 
-def _on_current_device(*tensors) -> None:
-    """Every tensor on the current GPU, whose stream and workspace a call uses."""
-    import torch
-    for t in tensors:
-        if not t.is_cuda or t.device.index != torch.cuda.current_device():
-            raise ValueError(f"tensor on {t.device}, not on the current GPU")
+def _pair(name: str, device: int, a, b) -> None:
+    """Two row tensors: the same dtype and shape, contiguous, on the current GPU
+    (whose stream and workspace a call uses)."""
+    if a.get_device() != device or b.get_device() != device:
+        raise ValueError(f"{name}: tensors on {a.device} and {b.device}, not on the current GPU")
+    if a.dtype != b.dtype or a.shape != b.shape:
+        raise ValueError(f"{name}: the row tensors differ in dtype or shape")
+    if not (a.is_contiguous() and b.is_contiguous()):
+        raise ValueError(f"{name}: rows must be contiguous")
 
 
-def _index_args(n: int, **tensors) -> None:
-    """int32 contiguous arrays of n rows (None: not given)."""
-    import torch
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if t.dtype != torch.int32 or not t.is_contiguous() or t.shape[0] != n:
-            raise ValueError(f"{name} must be a contiguous int32 tensor of {n} rows")
-        _on_current_device(t)
+def _index(name: str, device: int, t, n: int, dims: int = 1) -> int:
+    """Address of an int32 array of n entries (of dims 2, rows)."""
+    if t.dtype is not _int32 or t.dim() != dims or t.shape[0] != n or \
+            not t.is_contiguous() or t.get_device() != device:
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {dims} dimension(s), the "
+                         f"first of {n}, on the current GPU")
+    return t.data_ptr()
 
 
-def _cache_args(key_cache, value_cache, kv_heads: int, head_size: int, block_size: int | None):
+def _cache_args(device: int, key_cache, value_cache, kv_heads: int, head_size: int,
+                block_size: int | None):
     """(block_size, block stride, head stride) of a cache pair; the page size
     gives the block size where the caller does not."""
-    _on_current_device(key_cache, value_cache)
-    if key_cache.shape[1] != kv_heads:
-        raise ValueError(f"the cache has {key_cache.shape[1]} kv heads, not {kv_heads}")
-    if key_cache.element_size() != 1 or value_cache.element_size() != 1:
-        raise ValueError("a 4-bit cache is a uint8 tensor (kv4_cache_empty)")
-    if key_cache.shape != value_cache.shape or key_cache.stride() != value_cache.stride():
+    if key_cache.get_device() != device or value_cache.get_device() != device:
+        raise ValueError(f"caches on {key_cache.device} and {value_cache.device}, not on the "
+                         "current GPU")
+    shape, stride = key_cache.shape, key_cache.stride()
+    if key_cache.dtype is not _uint8 or value_cache.dtype is not _uint8 or len(shape) != 3:
+        raise ValueError("a 4-bit cache is a uint8 tensor of 3 dimensions (kv4_cache_empty)")
+    if shape != value_cache.shape or stride != value_cache.stride():
         raise ValueError("key_cache and value_cache differ in shape or strides")
-    page = key_cache.shape[2]
+    if shape[1] != kv_heads:
+        raise ValueError(f"the cache has {shape[1]} kv heads, not {kv_heads}")
+    page = shape[2]
+    if head_size <= 0:
+        raise ValueError(f"head_size {head_size}")
     if block_size is None:
         block_size = page // _page_bytes(head_size, 1)
-    if page != _page_bytes(head_size, block_size) or key_cache.stride(2) != 1:
+    if page != _page_bytes(head_size, block_size) or stride[2] != 1:
         raise ValueError(f"pages of {page} bytes do not hold whole tokens of head_size "
                          f"{head_size} and block_size {block_size}")
-    return block_size, key_cache.stride(0), key_cache.stride(1)
-
-
-def _rows_arg(name: str, key, value) -> None:
-    if key.dtype != value.dtype or key.shape != value.shape:
-        raise ValueError(f"{name}: key and value differ in dtype or shape")
-    if not (key.is_contiguous() and value.is_contiguous()):
-        raise ValueError(f"{name}: key and value rows must be contiguous")
-    _on_current_device(key, value)
+    return block_size, stride[0], stride[1]
 
 
 def paged_kv4_append(key_cache, value_cache, key, value, *, block_tables=None, positions=None,
@@ -110,24 +121,24 @@ def paged_kv4_append(key_cache, value_cache, key, value, *, block_tables=None, p
     (decode: row s is sequence s's token at positions[s]) through
     nxt_paged_kv4_append, or with slot_mapping (flat slot per row) through
     nxt_paged_kv4_write_slots.  No two rows of a call may have the same slot."""
-    lib = _lib.backend()
+    lib, dev = _lib.backend(), _current_device()
     num_tokens, kvh, head_size = key.shape
-    _rows_arg("paged_kv4_append", key, value)
-    bs, bstride, hstride = _cache_args(key_cache, value_cache, kvh, head_size, block_size)
-    _index_args(num_tokens, block_tables=block_tables, positions=positions,
-                slot_mapping=slot_mapping)
+    _pair("paged_kv4_append", dev, key, value)
+    bs, bstride, hstride = _cache_args(dev, key_cache, value_cache, kvh, head_size, block_size)
     dtype, st = kv_dtype_of(key), _stream_handle(stream)
     if slot_mapping is not None:
         status = lib.nxt_paged_kv4_write_slots(
-            _ptr(key_cache), _ptr(value_cache), _ptr(key), _ptr(value), _ptr(slot_mapping),
-            num_tokens, kvh, head_size, bs, bstride, hstride, dtype, st)
+            key_cache.data_ptr(), value_cache.data_ptr(), key.data_ptr(), value.data_ptr(),
+            _index("slot_mapping", dev, slot_mapping, num_tokens), num_tokens, kvh, head_size, bs,
+            bstride, hstride, dtype, st)
     else:
         if block_tables is None or positions is None:
             raise ValueError("need block_tables and positions, or slot_mapping")
         status = lib.nxt_paged_kv4_append(
-            _ptr(key_cache), _ptr(value_cache), _ptr(key), _ptr(value), _ptr(block_tables),
-            _ptr(positions), num_tokens, kvh, head_size, block_tables.shape[1], bs, bstride,
-            hstride, dtype, st)
+            key_cache.data_ptr(), value_cache.data_ptr(), key.data_ptr(), value.data_ptr(),
+            _index("block_tables", dev, block_tables, num_tokens, 2),
+            _index("positions", dev, positions, num_tokens), num_tokens, kvh, head_size,
+            block_tables.shape[1], bs, bstride, hstride, dtype, st)
     return _raise(lib, status, check)
 
 
@@ -135,15 +146,14 @@ def paged_kv4_read(key, value, key_cache, value_cache, slot_mapping, *,
                    block_size: int | None = None, stream=None, check: bool = True) -> int:
     """The values held in slot slot_mapping[i] into row i of key / value
     (nxt_paged_kv4_read_slots); a negative slot leaves its row as it was."""
-    lib = _lib.backend()
+    lib, dev = _lib.backend(), _current_device()
     num_tokens, kvh, head_size = key.shape
-    _rows_arg("paged_kv4_read", key, value)
-    bs, bstride, hstride = _cache_args(key_cache, value_cache, kvh, head_size, block_size)
-    _index_args(num_tokens, slot_mapping=slot_mapping)
+    _pair("paged_kv4_read", dev, key, value)
+    bs, bstride, hstride = _cache_args(dev, key_cache, value_cache, kvh, head_size, block_size)
     status = lib.nxt_paged_kv4_read_slots(
-        _ptr(key), _ptr(value), _ptr(key_cache), _ptr(value_cache), _ptr(slot_mapping),
-        num_tokens, kvh, head_size, bs, bstride, hstride, kv_dtype_of(key),
-        _stream_handle(stream))
+        key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+        _index("slot_mapping", dev, slot_mapping, num_tokens), num_tokens, kvh, head_size, bs,
+        bstride, hstride, kv_dtype_of(key), _stream_handle(stream))
     return _raise(lib, status, check)
 
 
@@ -152,37 +162,30 @@ def paged_kv4_copy_slots(key_cache, value_cache, src_slots, dst_slots, *, head_s
     """Copy the rows of page slots src_slots[i] to dst_slots[i] (int32 device
     tensors) inside the caches (nxt_paged_kv4_copy_slots): the copy-on-write of
     a partly shared page at admission."""
-    lib = _lib.backend()
-    bs, bstride, hstride = _cache_args(key_cache, value_cache, key_cache.shape[1], head_size,
-                                       block_size)
-    _index_args(src_slots.shape[0], src_slots=src_slots, dst_slots=dst_slots)
+    lib, dev = _lib.backend(), _current_device()
+    kvh, n = key_cache.shape[1], src_slots.shape[0]
+    bs, bstride, hstride = _cache_args(dev, key_cache, value_cache, kvh, head_size, block_size)
     status = lib.nxt_paged_kv4_copy_slots(
-        _ptr(key_cache), _ptr(value_cache), _ptr(src_slots), _ptr(dst_slots),
-        src_slots.shape[0], key_cache.shape[1], head_size, bs, bstride, hstride,
+        key_cache.data_ptr(), value_cache.data_ptr(), _index("src_slots", dev, src_slots, n),
+        _index("dst_slots", dev, dst_slots, n), n, kvh, head_size, bs, bstride, hstride,
         _stream_handle(stream))
     return _raise(lib, status, check)
 
 
 def paged_attention_kv4(out, query, key_cache, value_cache, block_tables, seq_lens, *,
                         num_kv_heads: int, scale: float, block_size: int | None = None,
-                        max_num_blocks_per_seq: int | None = None, stream=None,
-                        check: bool = True) -> int:
+                        stream=None, check: bool = True) -> int:
     """Decode attention over a 4-bit cache (nxt_paged_attention_kv4): as
     paged_attention, with K and V the values that the cache holds."""
-    lib = _lib.backend()
+    lib, dev = _lib.backend(), _current_device()
     num_seqs, num_heads, head_size = query.shape
-    if out.dtype != query.dtype or out.shape != query.shape:
-        raise ValueError("out and query differ in dtype or shape")
-    if not (out.is_contiguous() and query.is_contiguous()):
-        raise ValueError("query and out must be contiguous")
-    bs, bstride, hstride = _cache_args(key_cache, value_cache, num_kv_heads, head_size,
+    _pair("paged_attention_kv4", dev, out, query)
+    bs, bstride, hstride = _cache_args(dev, key_cache, value_cache, num_kv_heads, head_size,
                                        block_size)
-    _on_current_device(query, out)
-    _index_args(num_seqs, block_tables=block_tables, seq_lens=seq_lens)
-    if max_num_blocks_per_seq is None:
-        max_num_blocks_per_seq = block_tables.shape[1]
+    width = block_tables.shape[1]
     status = lib.nxt_paged_attention_kv4(
-        _ptr(out), _ptr(query), _ptr(key_cache), _ptr(value_cache), _ptr(block_tables),
-        _ptr(seq_lens), num_seqs, num_heads, head_size, num_kv_heads, ctypes.c_float(scale),
-        max_num_blocks_per_seq, bs, bstride, hstride, kv_dtype_of(query), _stream_handle(stream))
+        out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+        _index("block_tables", dev, block_tables, num_seqs, 2),
+        _index("seq_lens", dev, seq_lens, num_seqs), num_seqs, num_heads, head_size, num_kv_heads,
+        float(scale), width, bs, bstride, hstride, kv_dtype_of(query), _stream_handle(stream))
     return _raise(lib, status, check)
