@@ -68,6 +68,26 @@ def test_written_rows_read_back(cuda, d, dtype):
         _same(vo, wv)
 
 
+def test_step_is_rounded_twice(cuda):
+    """Ranges whose fifteenth, rounded to fp32 on its way to fp16, is not the fp16
+    number nearest to it."""
+    g = torch.Generator().manual_seed(15)
+    x = torch.randn((400000, 32), generator=g)
+    span = (x.max(1).values - x.min(1).values).numpy()
+    exact = span.astype(np.float64) * np.float64(np.float32(1.0 / 15.0))
+    pick = exact.astype(np.float16) != exact.astype(np.float32).astype(np.float16)
+    assert pick.sum() >= 5
+    k = x[torch.from_numpy(pick)][:, None].contiguous()
+    n = k.shape[0]
+    kc, vc = _cache(-(-n // 16), 1, 32, 16)
+    slots = np.arange(n, dtype=np.int32)
+    _write(kc, vc, k, k, slots)
+    ko, vo = (torch.empty((n, 1, 32), device="cuda") for _ in "kv")
+    KV4.paged_kv4_read(ko, vo, kc, vc, _dev(slots))
+    _same(ko, _stored(k, "fp32"))
+    _same(vo, _stored(k, "fp32"))
+
+
 @pytest.mark.parametrize("bs", [16, 64, 1024])
 def test_append_by_tables(cuda, bs):
     """Tokens at the edges of pages and tiles; skipped positions; other slots

@@ -57,6 +57,14 @@ template <int KV> __device__ __forceinline__ void store_piece(void *rows, size_t
     }
 }
 
+// x as the fp32 number that it is: a conversion to fp16 behind it is a rounding of
+// its own (the compiler joins it with the product in one instruction, which
+// rounds once).
+__device__ __forceinline__ float rounded(float x) {
+    asm("" : "+v"(x));
+    return x;
+}
+
 // Codes, low and step of one group whose 8-channel pieces lie in the lanes of
 // a quad (piece_ok: the piece is inside head_size; else its codes are 0).
 struct Kv4Piece {
@@ -85,7 +93,7 @@ __device__ __forceinline__ Kv4Piece quantise(const float (&in)[8], bool piece_ok
     hi = fmaxf(hi, dpp_mov<0x4E>(hi));
     const int lane = threadIdx.x & 63;
     nan = ((__ballot(nan) >> (lane & ~3)) & 15) != 0;
-    const _Float16 low = (_Float16)lo, step = (_Float16)((hi - lo) * (1.0f / 15.0f));
+    const _Float16 low = (_Float16)lo, step = (_Float16)rounded((hi - lo) * (1.0f / 15.0f));
     const float lowf = (float)low, stepf = (float)step;
     const float inv = 1.0f / stepf;
     const bool live = piece_ok && !nan && stepf > 0.0f;
