@@ -58,14 +58,17 @@ def attention_bound(dtype, out, size, spread):
     32 elements of a group at once, under 2^-17 of spread between them in all;
     and the rounded score itself and the exponential, 2^-22 of the spread and
     2^-22.  An error e of the scores moves an output by at most 2e * size.
-    A weight goes to the matrix product times its step, and alone times the
-    low, rounded to fp16 (bf16 output: 2^-11) or to two fp16 parts (2^-21),
-    and the sum over the tokens adds 2^-20 at most (64 roundings of partial
+    A weight p is rounded to fp16 (bf16 output: by 2^-11 of it) or to two fp16
+    parts (2^-22), and these weights are the ones that are summed to divide by:
+    with p' = p (1 + e), |e| <= u, the quotient sum p' v / sum p' moves by
+    sum p e (v - out) / sum p' <= u (size + |out|) <= 2 u size.  Times its step
+    it is rounded once more, by the same u of step * code: 3 u size in all.
+    And the sum over the tokens adds 2^-20 at most (64 roundings of partial
     sums, several chains).  Then the output's own rounding: half a step of its
     value, and for fp16 at least half of the subnormal unit 2^-24 (an output of
     3e-5 is 2^-15.02 and is held as a multiple of 2^-24, so it is off by up to
     2^-25 whatever computed it)."""
-    weight = 2.0 ** -11 if dtype == "bf16" else 2.0 ** -21
+    weight = 3 * (2.0 ** -11 if dtype == "bf16" else 2.0 ** -22)
     e = (2.0 ** -17) * spread[..., None] + 2.0 ** -21
     rounding = np.maximum(HALF_STEP[dtype] * np.abs(out), 2.0 ** -25 if dtype == "fp16" else 0.0)
     return rounding + (weight + 2.0 ** -20 + 2 * e) * size + 1e-30

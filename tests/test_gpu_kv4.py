@@ -241,6 +241,53 @@ def test_groups_of_query_heads(cuda, dtype, group):
     _check(_attend(q, kc, vc, bt, lens, 2), dtype, C.reference(q, k, v, lens, C.scale_of(128), 2))
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("h,kvh,d,bs", [(32, 2, 128, 16), (18, 2, 64, 16), (16, 1, 32, 16),
+                                        (12, 1, 80, 32), (44, 4, 112, 16), (40, 1, 192, 16)])
+def test_larger_groups_with_cut_segments(cuda, dtype, h, kvh, d, bs):
+    """Groups of 9 to 40 heads: segments over many workgroups, inside one, and
+    several in one wavefront's range (2400 sequences of 1 to 160 tokens)."""
+    lens = [3000, 900] + RAGGED + [1 + (i * 37) % 160 for i in range(2400)] + [2100]
+    q, k, v, kc, vc, bt = _batch(dtype, h, kvh, d, bs, lens, seed=h)
+    out = _attend(q, kc, vc, bt, lens, kvh)
+    pick = list(range(0, len(lens), 43)) + [1, len(lens) - 1]
+    starts = np.concatenate([[0], np.cumsum(lens)[:-1]])
+    ref = C.reference(q[pick], k, v, [lens[i] for i in pick], C.scale_of(d), kvh, starts[pick])
+    _check(out[pick], dtype, ref)
+    for _ in range(5):
+        assert torch.equal(_attend(q, kc, vc, bt, lens, kvh), out)
+
+
+def test_larger_groups_with_nan_and_missing_pages(cuda):
+    """A NaN query, NaN values and pages that are not there stay with their heads
+    and sequences where pieces are joined."""
+    kvh, d, bs = 2, 128, 16
+    lens = [500, 40, 100] + [1 + (i * 29) % 150 for i in range(2200)]
+    q, k, v, kc, vc, bt = _batch("fp16", 16 * kvh, kvh, d, bs, lens, seed=1)
+    want = _attend(q, kc, vc, bt, lens, kvh)
+    q2, cut = q.clone(), bt.copy()
+    q2[0, 5, 7] = float("nan")
+    q2[900, 20] = float("inf")
+    cut[1, :] = -1
+    cut[2, 3:] = -1
+    v2 = v[:lens[0]].clone()
+    v2[480, 1, 100] = float("nan")
+    _write(kc, vc, k[:lens[0]], v2, C.slots_for(bt[:1], lens[:1], bs))
+    out = _attend(q2, kc, vc, cut, lens, kvh)
+    assert torch.isnan(out[0, 5]).all() and torch.isnan(out[900, 20]).all()
+    assert torch.isnan(out[0, 16:, 96:]).all()
+    assert bool((out[1] == 0).all())
+    starts = np.concatenate([[0], np.cumsum(lens)[:-1]])
+    ref = C.reference(q[2:3], k, v, [3 * bs], C.scale_of(d), kvh, starts[2:3])
+    _check(out[2:3], "fp16", ref)
+    # (the step of a NaN row lowers the weights' scale for its kv head: other bits)
+    ref = C.reference(q[:1], k, v, lens[:1], C.scale_of(d), kvh, starts[:1])
+    _check(out[:1, 16:, :96], "fp16", [r[:, 16:, :96] if r.ndim == 3 else r[:, 16:] for r in ref])
+    same = torch.ones_like(out, dtype=torch.bool)
+    same[0, 5], same[900, 20], same[1], same[2], same[0, 16:] = (False,) * 5
+    assert torch.equal(out[same], want[same])
+
+
 @pytest.mark.parametrize("dtype,d", [("fp16", 128), ("bf16", 256), ("fp32", 64), ("fp32", 256)])
 def test_one_long_sequence(cuda, dtype, d):
     """Split over the whole GPU, with keys that make sharp peaks."""

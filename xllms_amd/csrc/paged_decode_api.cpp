@@ -1210,6 +1210,7 @@ int kv4_attention_run(void *out, const void *query, const void *key_cache, const
         p.min_tiles_per_wave = kKv4MinTiles;
         p.seg_cost = kKv4SegmentCost;
         p.segment_split = 1;
+        p.wg_fix = xhip::kv4_wg_fix(head_tile, group, head_size) ? 1 : 0;
         p.merge_per_segment = merge_per_segment(group, head_tile, head_size, nseq, segs, cus);
         p.wg_trace = t_wg_trace;
         const auto launch = dtype == NXT_KV_FP16   ? xhip::launch_kv4_f16

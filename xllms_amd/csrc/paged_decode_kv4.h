@@ -481,6 +481,86 @@ __device__ __forceinline__ void kv4_write(const DecodeParams &p, const MfmaPiece
     }
 }
 
+// Cut segments (wg_fix).  The wavefronts of a workgroup own consecutive ranges,
+// so a segment's pieces in one workgroup are joined in it: a wavefront whose
+// last piece continues its left neighbour's leaves its state in LDS, where the
+// tiles were, and after a barrier the leftmost holder of each segment takes its
+// neighbours' states, writes the rows if that was the whole segment, and else
+// one partial.  (A cut first piece with others behind it, whose wavefront needs
+// its slots still, goes to memory as a partial at once, and is taken from there.)
+// (kv4_wg_fix: not with split columns, nor for two row blocks, whose states do
+// not fit the slots.)
+template <int D> struct Kv4FixSlot {
+    f32x4 o[Kv4Geometry<D>::NG][2][64], low[64];
+    float base[64], limit[64];
+};
+
+template <int D>
+__device__ __forceinline__ void kv4_fix_store(Kv4FixSlot<D> &to, int lane, const Kv4State<D> &st) {
+#pragma unroll
+    for (int g = 0; g < Kv4Geometry<D>::NG; g++) {
+        to.o[g][0][lane] = st.o[g][0];
+        to.o[g][1][lane] = st.o[g][1];
+    }
+    to.low[lane] = st.low;
+    to.base[lane] = st.base;
+    to.limit[lane] = st.limit;
+}
+
+// Brings st to the larger of its base and another state's and returns the
+// factor of that state's sums.  A state before its first score (limit -inf) has
+// sums of zero, or of NaN, which stay.
+template <int D> __device__ __forceinline__ float kv4_rebase(Kv4State<D> &st, float base, bool fresh) {
+    const bool own_fresh = st.limit == -INFINITY;
+    const float top = own_fresh ? base : fresh ? st.base : fmaxf(st.base, base);
+    const float own = own_fresh ? 1.0f : fast_exp2(st.base - top);
+    st.low *= own;
+#pragma unroll
+    for (int g = 0; g < Kv4Geometry<D>::NG; g++) {
+        st.o[g][0] *= own;
+        st.o[g][1] *= own;
+    }
+    st.base = top;
+    if (!fresh) st.limit = 0.0f;  // (any but -inf: no more scores come)
+    return fresh ? 1.0f : fast_exp2(base - top);
+}
+
+template <int D>
+__device__ __forceinline__ void kv4_fix_absorb(const Kv4FixSlot<D> &from, int lane, Kv4State<D> &st) {
+    const float w = kv4_rebase<D>(st, from.base[lane], from.limit[lane] == -INFINITY);
+#pragma unroll
+    for (int g = 0; g < Kv4Geometry<D>::NG; g++) {
+        st.o[g][0] += from.o[g][0][lane] * w;
+        st.o[g][1] += from.o[g][1][lane] * w;
+    }
+    st.low += from.low[lane] * w;
+}
+
+// The same from the partial in a slot of the workspace.
+template <int D>
+__device__ __forceinline__ void kv4_fix_absorb(const DecodeParams &p, const MfmaPiece &pc, int slot, int lane,
+                                               Kv4State<D> &st) {
+    constexpr int NG = Kv4Geometry<D>::NG;
+    const int j = lane & 15, q = lane >> 4;
+    if (j >= min(kMfmaHeads, p.group - pc.ht * kMfmaHeads)) return;  // (never written)
+    const size_t row = (size_t)slot * kMfmaHeads + j;
+    const float m = p.ws_ml[row * 2], l = p.ws_ml[row * 2 + 1];
+    const float w = kv4_rebase<D>(st, m, m == -INFINITY);
+    st.low[NG & 3] += q == NG >> 2 ? l * w : 0.0f;
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        const int c = 32 * g + 8 * q;
+        if (D % 32 != 0 && c >= D) continue;
+        float f[8];
+        load_floats(p.ws_o + row * D + c, f);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            st.o[g][0][i] += f[2 * i] * (w * (1.0f / 16777216.0f));
+            st.o[g][1][i] += f[2 * i + 1] * (w * (1.0f / 1048576.0f));
+        }
+    }
+}
+
 // One tile of a wavefront's range: where its two cache tiles are, in bytes from
 // the start of either cache, and whether their pages are there.
 struct Kv4TileRef {
@@ -566,10 +646,18 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D))) void paged
     constexpr int kX = SPLIT ? 4 : 8;  // scores of a lane
     static_assert(!SPLIT || R == 1, "split columns: one block");
     extern __shared__ int pre[];  // num_seqs + 1 split-unit prefixes
-    __shared__ __attribute__((aligned(16))) char slots[kKv4Waves][S][G::kSlot];
+    constexpr bool FIX = kv4_wg_fix(kMfmaHeads * R, SPLIT ? 1 : kMfmaHeads, D);
+    // a wavefront's tiles, and its state at the end
+    constexpr int kWaveLds = S * G::kSlot > (int)sizeof(Kv4FixSlot<D>) || !FIX ? S * G::kSlot : (int)sizeof(Kv4FixSlot<D>);
+    __shared__ __attribute__((aligned(16))) char slots[kKv4Waves][kWaveLds];
+    // what a wavefront has of its left neighbour's last segment: nothing, a state in
+    // LDS that the next wavefront continues, one that ends the segment, or a partial
+    // in memory (which ends it)
+    enum { kNothing, kOpen, kEnd, kStored };
+    __shared__ int continues[FIX ? kKv4Waves : 1];
     XHIP_WG_BEGIN(p);
     if (threadIdx.x < S * kKv4Waves)  // (the fetches leave them alone)
-        *(u32x4 *)&slots[threadIdx.x / S][threadIdx.x % S][G::kOnes] =
+        *(u32x4 *)&slots[threadIdx.x / S][threadIdx.x % S * G::kSlot + G::kOnes] =
             u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
     batch_prefix<TT, kKv4Waves>(p, pre);
     XHIP_WG_STAMP(p, 1);
@@ -600,13 +688,16 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D))) void paged
     const RangeCursor start = cur;
     MfmaPiece pc;
     bool has_next = next_piece<TT>(p, lens, pre, cur, pc);
+    Kv4State<D> st[R];
+    bool have_last = false;  // of a cut piece, in st
+    int cont = kNothing;
     if (has_next) {
         Kv4Walker<D> ahead;
         ahead.cur = start;
         ahead.piece(p, lens, tables, pre);
         // LDS address of the wavefront's slots, K half then V half of each
         const uint32_t lds0 =
-            (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)&slots[wave][0][0];
+            (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)&slots[wave][0];
         Kv4TileRef ref[S];  // the tile at hand and those behind it
 #pragma unroll
         for (int i = 0; i < S; i++) {
@@ -618,10 +709,9 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D))) void paged
         const int low_a = j < NG ? 2 * G::kBytes + kv4_v_low(NG, 4 * q, j < NG ? j : 0) : G::kOnes;
         const int low_b = j < NG ? low_a + G::kBytes : G::kOnes;
         int slot = 0;
-        if (threadIdx.x < 64 * kMfmaWavesPerGroup) XHIP_WAVE_STAMP(p, threadIdx.x >> 6, 0);  // (a record holds four)
+        XHIP_WAVE_STAMP(p, wave, 0);
         while (has_next) {
             Kv4Query<KV, D, SPLIT> qr[R];
-            Kv4State<D> st[R];
             const int g0 = pc.ht * kMfmaHeads * R;
             float limit = kKv4Limit;
             uint32_t big_step = kKv4BigStep;
@@ -636,7 +726,8 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D))) void paged
             }
             for (int t0 = pc.t_begin; t0 < pc.t_end; t0 += TT) {
                 const Kv4TileRef nx = ahead.take(p, lens, tables, pre);
-                const char *ks = &slots[wave][slot][0], *vs = ks + 2 * G::kBytes;
+                char *ks = &slots[wave][slot * G::kSlot];
+                const char *vs = ks + 2 * G::kBytes;
                 const uint32_t lds = lds0 + (uint32_t)(slot * G::kSlot);
                 float x[R][kX];
                 kv4_wait<(2 * S - 1) * NF>();  // later: this tile's V, K and V of the next S - 1
@@ -651,7 +742,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D))) void paged
                         const int n = (h ? ref[0].b : ref[0].a) ? pc.t_end - t0 - 16 * h : 0;  // tokens
                         for (int i = lane; i < 16 * NG; i += 64)
                             if (i / NG >= n)
-                                *(uint16_t *)(slots[wave][slot] + h * G::kBytes + kv4_k_low(NG, i / NG, i % NG)) = 0;
+                                *(uint16_t *)(ks + h * G::kBytes + kv4_k_low(NG, i / NG, i % NG)) = 0;
                     }
                     wave_lds_fence();  // before the reads below, by other lanes
                 }
@@ -675,7 +766,7 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D))) void paged
 #pragma unroll
                                 for (int b = 0; b < R; b++) keep_score(x[b][4 * h + e], 4 * q + e < m);
                         }
-                        uint16_t *t = (uint16_t *)(slots[wave][slot] + (2 + h) * G::kBytes);
+                        uint16_t *t = (uint16_t *)(ks + (2 + h) * G::kBytes);
                         for (int i = lane; i < 16 * NG; i += 64) {
                             if ((i / (4 * NG)) * 4 + (i & 3) < n) continue;
                             t[kv4_step(NG, 0, 0) / 2 + i] = 0;
@@ -738,11 +829,38 @@ __global__ __launch_bounds__(64 * kKv4Waves, (kv4_waves_per_simd(D))) void paged
                 ref[S - 1] = nx;
                 slot = slot + 1 == S ? 0 : slot + 1;
             }
+            MfmaPiece next = pc;
+            has_next = next_piece<TT>(p, lens, pre, cur, next);
+            have_last = FIX && !has_next && !pc.whole;
+            if (have_last) break;
+            if (FIX && !pc.whole && pc.t_begin > 0) cont = kStored;
             kv4_write<KV, D, R>(p, pc, lane, st);
-            has_next = next_piece<TT>(p, lens, pre, cur, pc);
+            pc = next;
         }
-        if (threadIdx.x < 64 * kMfmaWavesPerGroup) XHIP_WAVE_STAMP(p, threadIdx.x >> 6, 1);
+        XHIP_WAVE_STAMP(p, wave, 1);
         kv4_wait<0>();  // nothing of this wavefront's may reach LDS after its end
+    }
+    if constexpr (FIX) {
+        if (have_last && wave > 0 && pc.t_begin > 0) {
+            kv4_fix_store<D>(*(Kv4FixSlot<D> *)slots[wave], lane, st[0]);
+            cont = pc.t_end < pc.L ? kOpen : kEnd;
+            have_last = false;
+        }
+        if (lane == 0) continues[wave] = cont;
+        __syncthreads();
+        if (have_last) {
+            bool ends = pc.t_end >= pc.L;
+            for (int k = wave + 1; k < kKv4Waves && !ends; k++) {
+                const int c = __builtin_amdgcn_readfirstlane(continues[k]);
+                if (c == kStored)
+                    kv4_fix_absorb<D>(p, pc, (w - wave + k) * 2, lane, st[0]);
+                else
+                    kv4_fix_absorb<D>(*(const Kv4FixSlot<D> *)slots[k], lane, st[0]);
+                ends = c != kOpen;
+            }
+            pc.whole = ends && pc.t_begin == 0;
+            kv4_write<KV, D, R>(p, pc, lane, st);
+        }
     }
     XHIP_WG_FLUSH(p);
 }
@@ -759,10 +877,8 @@ static hipError_t launch_kv4_kernel(const DecodeParams &p, hipStream_t st, hipEv
                             p.block_tables);
 }
 
-// Groups of up to 8 heads: the columns of the score products hold them twice,
-// for a tile's two cache tiles, so that a lane has 4 scores and not 8.
-constexpr int kKv4SplitHeads = 8;
-
+// (split columns: the score products hold the heads twice, for a tile's two cache
+// tiles, so that a lane has 4 scores and not 8)
 template <int KV, int D>
 static hipError_t launch_kv4_size(const DecodeParams &p, int head_tile, hipStream_t st,
                                   hipEvent_t ev_start, hipEvent_t ev_stop) {
@@ -773,9 +889,12 @@ static hipError_t launch_kv4_size(const DecodeParams &p, int head_tile, hipStrea
             return launch_merge<KV, D, 2 * kMfmaHeads, kKv4TileTokens>(p, st);
         }
     }
-    const hipError_t e = p.group <= kKv4SplitHeads
-                             ? launch_kv4_kernel<KV, D, 1, true>(p, st, ev_start, ev_stop)
-                             : launch_kv4_kernel<KV, D, 1, false>(p, st, ev_start, ev_stop);
+    hipError_t e;
+    if constexpr (kv4_split(1, D))
+        e = kv4_split(p.group, D) ? launch_kv4_kernel<KV, D, 1, true>(p, st, ev_start, ev_stop)
+                                  : launch_kv4_kernel<KV, D, 1, false>(p, st, ev_start, ev_stop);
+    else
+        e = launch_kv4_kernel<KV, D, 1, false>(p, st, ev_start, ev_stop);
     if (e != hipSuccess) return e;
     return launch_merge<KV, D, kMfmaHeads, kKv4TileTokens>(p, st);
 }
@@ -796,9 +915,10 @@ template <int KV, int D> static const void *kv4_fn(int head_tile, int group) {
     if constexpr (kv4_has_wide(D))
         if (head_tile == 2 * kMfmaHeads)
             return reinterpret_cast<const void *>(&paged_decode_partition_kv4_kernel<KV, D, 2, false>);
-    return group <= kKv4SplitHeads
-               ? reinterpret_cast<const void *>(&paged_decode_partition_kv4_kernel<KV, D, 1, true>)
-               : reinterpret_cast<const void *>(&paged_decode_partition_kv4_kernel<KV, D, 1, false>);
+    if constexpr (kv4_split(1, D))
+        if (kv4_split(group, D))
+            return reinterpret_cast<const void *>(&paged_decode_partition_kv4_kernel<KV, D, 1, true>);
+    return reinterpret_cast<const void *>(&paged_decode_partition_kv4_kernel<KV, D, 1, false>);
 }
 
 template <int KV> static int kv4_occupancy_dtype(int head_size, int head_tile, int group, size_t lds_bytes) {

@@ -66,6 +66,26 @@ constexpr int mfma_wg_fixup(int rows_per_tile, int head_size) {
     return head_size > 192 ? 0 : rows_per_tile == kMfmaHeads ? 1 : 2;
 }
 
+// Whether the partition kernel of a 4-bit cache splits its score columns between
+// two cache tiles: groups of up to 8 heads, head sizes whose second set of query
+// operands fits the registers.  32 / 8 heads, 64 sequences of 512-4096 tokens, us
+// a step split and not: head_size 128 fp16 55.1 and 57.9, bf16 53.8 and 55.6,
+// fp32 55.5 and 58.4; 64 fp16 43.5 and 42.9; 32 fp16 37.0 and 38.2; 256 fp16 97.3
+// and 98.4, fp32 99.5 and 99.8; 192 fp16 75.1 and 74.3, fp32 (spilled) 82.9 and
+// 74.0.
+constexpr bool kv4_split(int group, int head_size) { return group <= 8 && head_size <= 128; }
+
+// The same combine in that kernel, in the LDS where a wavefront's tiles were: for
+// one row block without split columns, where the joined state leaves the registers
+// of the main loop alone (not at head_size 192).  64 / 4 heads of 128, 128
+// sequences of 128-8192 tokens, bf16: 49.0 us a step with it, 52.0 without (the
+// merge 4.6 of it, 8.5 without).  The partials of few heads are small and the
+// barrier costs more: 32 / 8 heads, 64 sequences of 512-4096, fp16, 55.4 us with,
+// 54.2 without.
+constexpr bool kv4_wg_fix(int rows_per_tile, int group, int head_size) {
+    return rows_per_tile == kMfmaHeads && !kv4_split(group, head_size) && head_size <= 128;
+}
+
 // Wavefronts per SIMD of the MFMA partition kernel, which the automatic plan
 // launches in one resident round, by the bytes of a K (or V) row: about 64 KB
 // of tiles per CU, twice that with the next tiles in flight.  Rows of 128 to
