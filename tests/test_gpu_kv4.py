@@ -337,6 +337,47 @@ def test_queries_far_from_one(cuda, dtype, exp):
     _check(_attend(q, kc, vc, bt, lens, 1, scale=scale), dtype, C.reference(q, k, v, lens, scale, 1))
 
 
+@pytest.mark.parametrize("h,kvh,d", [(12, 12, 64), (8, 2, 128), (32, 2, 128), (24, 1, 96)])
+def test_fp32_keeps_its_bits(cuda, h, kvh, d):
+    """Root mean square error of fp32 outputs.  Scores of parts below 32 (log2
+    units) take about five roundings of at most 2^-20 each, 2^-20.8 rms, which
+    move the weights by ln 2 of that, independently: sqrt(5) * 2^-21.3 = 2^-20.2
+    of the output; and the sums' own, 2^-26 of the sizes, which are below 64
+    outputs here: 2^-20.  Together 2^-19.1."""
+    lens = [1000, 517, 1000, 64]
+    g = torch.Generator().manual_seed(d + h)
+    q = 0.25 * torch.randn((len(lens), h, d), generator=g)
+    k, v = (torch.randn((sum(lens), kvh, d), generator=g) for _ in "kv")
+    bt, pool = C.tables_for(lens, 16, 0)
+    kc, vc = _cache(pool, kvh, d, 16, fill=0xFF)
+    _write(kc, vc, k, v, C.slots_for(bt, lens, 16))
+    ref = C.reference(q, k, v, lens, C.scale_of(d), kvh)
+    assert ref[2].max() * np.log2(np.e) < 32
+    err = C.np64(_attend(q, kc, vc, bt, lens, kvh)) - ref[0]
+    rel = np.sqrt((err ** 2).mean() / (ref[0] ** 2).mean())
+    print(f"rms {rel:.2e}")
+    assert rel < 2.0 ** -19
+
+
+def test_long_ranges_do_not_drift(cuda):
+    """8192 tokens times 2000 sequences of one set of pages: whole sequences in a
+    wavefront's range, nearly equal weights, outputs far below the values."""
+    n, d = 2000, 32
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.randn((8192, 1, d), generator=g) for _ in "kv")
+    bt, pool = C.tables_for([8192], 16, 0)
+    for dtype, most in (("fp32", 1e-4), ("fp16", 2.0 ** -12 + 1e-4)):
+        q = (0.1 * torch.randn((n, 2, d), generator=g)).to(C.DTYPES[dtype])
+        kd, vd = k.to(C.DTYPES[dtype]), v.to(C.DTYPES[dtype])
+        kc, vc = _cache(pool, 1, d, 16)
+        _write(kc, vc, kd, vd, C.slots_for(bt, [8192], 16))
+        out = _attend(q, kc, vc, np.repeat(bt, n, 0), [8192] * n, 1)
+        ref = C.reference(q[:3], kd, vd, [8192] * 3, C.scale_of(d), 1, [0, 0, 0])[0]
+        rel = np.sqrt(((C.np64(out[:3]) - ref) ** 2).mean() / (ref ** 2).mean())
+        print(f"{dtype} rms {rel:.2e}")
+        assert rel < most
+
+
 def test_queries_of_zero(cuda):
     lens = [33]
     q, k, v, kc, vc, bt = _batch("fp16", 4, 2, 64, 16, lens)
