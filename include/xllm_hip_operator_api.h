@@ -291,8 +291,8 @@ int nxt_paged_kv_copy_slots(void *key_cache, void *value_cache, const int *src_s
  * call to call on one cache.
  * All calls are asynchronous on `stream` and return NXT_ATTN_OK or a negative
  * status (also recorded for nxt_attn_last_status); a refused call launches
- * nothing.  The caller owns every buffer and guarantees that page ids and
- * slots lie inside the cache. */
+ * nothing.  Caches, rows, query and out are 16-byte aligned.  The caller owns
+ * every buffer and guarantees that page ids and slots lie inside the cache. */
 
 /* Bytes of one page of one kv head (of K, and as many of V), or a negative
  * status. */
@@ -338,7 +338,13 @@ int nxt_paged_kv4_copy_slots(void *key_cache, void *value_cache, const int *src_
 /* nxt_paged_attention_ex over a 4-bit cache: the same computation and contract
  * points (empty sequences, negative page ids, lengths past the table, slots
  * past the length) with K_t and V_t the values stored; query and out in dtype.
- * num_heads / num_kv_heads <= 64. */
+ * num_heads / num_kv_heads <= 64.  A query row with an infinity or a NaN, and a
+ * head that meets a NaN row, come out as NaN; other rows keep their values.  The
+ * error beyond out's own rounding is that of fp32 sums of the terms
+ * p (step code) and p low one by one (whose sizes are those of the range, not of
+ * the value), for fp16 and bf16 up to 2^-18 of them, and for bf16 that of weights
+ * rounded to fp16.  The workspace is the decode calls': a call that is to be
+ * captured into a graph is made once before, on its stream, at its shape. */
 int nxt_paged_attention_kv4(void *out, const void *query, const void *key_cache,
                             const void *value_cache, const int *block_tables,
                             const int *seq_lens, int num_seqs, int num_heads, int head_size,

@@ -50,8 +50,8 @@
 // own waits for LDS loads in flight would drain them all.
 //
 // Per 32 tokens of a kv head at head_size 128 that is 5120 bytes, about 210
-// vector instructions (fp16; bf16 165) and 28 (bf16, whole columns) to 37 (fp16,
-// split columns) MFMAs.  With everything in LDS already the two kinds take 72%
+// vector instructions (fp16 in split columns) and 28 MFMAs (bf16 in whole
+// columns: 19).  With everything in LDS already the two kinds take 72%
 // and 28% of the time, one after the other: a wavefront's tile is a chain.  The
 // fetches alone reach 5.9-6.1 TB/s, the kernel 5.4 over a large batch (256
 // sequences of 512-8192 tokens, 32 / 8 heads of 128, fp16, 1.43 GB in 271 us with
