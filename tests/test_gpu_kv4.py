@@ -298,6 +298,23 @@ def test_one_long_sequence(cuda, dtype, d):
     _check(_attend(q, kc, vc, bt, lens, 1), dtype, C.reference(q, k, v, lens, C.scale_of(d), 1))
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("h,d", [(4, 128), (16, 128), (32, 64), (4, 80), (16, 192), (8, 256)])
+def test_long_ranges(cuda, dtype, h, d):
+    """Ranges of dozens of tiles, that end anywhere, in every form of the kernel."""
+    n, L = 1500, 2047
+    q = C.rows(n, h, d, dtype, 1)
+    k, v = C.rows(L, 1, d, dtype, 2), C.rows(L, 1, d, dtype, 3)
+    bt, pool = C.tables_for([L], 16, 0)
+    kc, vc = _cache(pool, 1, d, 16, fill=0xFF)
+    _write(kc, vc, k, v, C.slots_for(bt, [L], 16))
+    lens = [L - 3 * (i % 50) for i in range(n)]
+    out = _attend(q, kc, vc, np.repeat(bt, n, 0), lens, 1)
+    pick = [0, 49, 700, n - 1]
+    ref = C.reference(q[pick], k, v, [lens[i] for i in pick], C.scale_of(d), 1, [0] * len(pick))
+    _check(out[pick], dtype, ref)
+
+
 def test_many_sequences(cuda):
     """More sequences than one launch takes."""
     lens = [1 + (i * 7) % 40 for i in range(8200)]
@@ -376,6 +393,16 @@ def test_long_ranges_do_not_drift(cuda):
         rel = np.sqrt(((C.np64(out[:3]) - ref) ** 2).mean() / (ref ** 2).mean())
         print(f"{dtype} rms {rel:.2e}")
         assert rel < most
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_query_and_scale_far_apart(cuda, dtype):
+    """A scale whose product with a constant alone would pass fp32's range."""
+    lens = [70]
+    q, k, v, kc, vc, bt = _batch(dtype, 4, 1, 128, 16, lens, seed=6)
+    q = (q.double() * 2.0 ** -112).to(q.dtype)
+    scale = C.scale_of(128) * 2.0 ** 112
+    _check(_attend(q, kc, vc, bt, lens, 1, scale=scale), dtype, C.reference(q, k, v, lens, scale, 1))
 
 
 def test_queries_of_zero(cuda):

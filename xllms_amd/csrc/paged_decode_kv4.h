@@ -151,7 +151,8 @@ __device__ __forceinline__ void keep_score(float &x, bool ok) {
 // to 10 above its leading bit: a sum is right to ~2^-19 of its largest product,
 // always cut towards zero.  Under the rounding of a 16-bit output that goes;
 // for fp32 they are made normal numbers first, which is one multiplication a word.
-template <int KV> constexpr float kv4_code_scale() { return KV == KV_F32 ? 0x1p-9f : 0x1p-24f; }
+template <int KV> constexpr int kv4_code_exp() { return KV == KV_F32 ? 9 : 24; }
+template <int KV> constexpr float kv4_code_scale() { return 1.0f / (1 << kv4_code_exp<KV>()); }
 
 template <int KV, bool HIGH> __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
     w &= HIGH ? 0x00f000f0u : 0x000f000fu;
@@ -256,7 +257,7 @@ __device__ __forceinline__ void kv4_load_query(const DecodeParams &p, const Mfma
                              : u32x2{half_pair(s4[0] - r01.x, s4[1] - r01.y), half_pair(s4[2] - r23.x, s4[3] - r23.y)};
     o.sums[0] = sums & first;
     if constexpr (SPLIT) o.sums[1] = sums & ~first;
-    o.a = __builtin_amdgcn_ldexpf(p.scale_log2 * (1.0f / kv4_code_scale<KV>()), ex - 15);
+    o.a = __builtin_amdgcn_ldexpf(p.scale_log2, ex - 15 + kv4_code_exp<KV>());
     o.b = __builtin_amdgcn_ldexpf(p.scale_log2, ex - 15 + 9);
 }
 
