@@ -610,6 +610,43 @@ def test_refused_calls_leave_the_output(cuda):
     assert bool((out == 7.0).all())
 
 
+def test_more_refusals(cuda):
+    q, k, v, kc, vc, bt = _batch("fp16", 4, 2, 64, 16, [20])
+    row = torch.zeros((2, 2, 64), dtype=torch.float16, device="cuda")
+    slot = torch.zeros(2, dtype=torch.int32, device="cuda")
+    before = kc.clone()
+    wide = torch.empty((2, (1 << 31) // KV4.kv4_page_bytes(64, 16) + 1, kc.shape[2]), dtype=torch.uint8,
+                       device="cuda").transpose(0, 1)  # a head's pages past 2 GiB
+    for call in (lambda: KV4.paged_kv4_append(wide, wide, row, row, slot_mapping=slot),
+                 lambda: KV4.paged_kv4_append(kc, vc, row, row, slot_mapping=slot[:, None]),
+                 lambda: KV4.paged_kv4_append(kc, vc, row, row, block_tables=slot, positions=slot),
+                 lambda: KV4.paged_kv4_append(kc, vc, row[..., :0], row[..., :0], slot_mapping=slot),
+                 lambda: KV4.paged_kv4_append(kc, vc, row.cpu(), row.cpu(), slot_mapping=slot),
+                 lambda: KV4.paged_kv4_append(kc, vc, row, row, slot_mapping=slot.cpu()),
+                 lambda: KV4.paged_kv4_append(kc.cpu(), vc.cpu(), row, row, slot_mapping=slot),
+                 lambda: KV4.paged_kv4_copy_slots(kc, vc, slot, slot[:1], head_size=64),
+                 lambda: KV4.paged_kv4_copy_slots(kc, vc, slot, slot, head_size=128, block_size=16),
+                 lambda: KV4.paged_attention_kv4(row, row, kc, vc, slot, slot, num_kv_heads=2, scale=1.0)):
+        with pytest.raises(ValueError):
+            call()
+    assert torch.equal(kc, before)
+
+
+def test_no_rows_from_python(cuda):
+    kc, vc = _cache(2, 2, 64, 16)
+    before = kc.clone()
+    row = torch.zeros((0, 2, 64), dtype=torch.bfloat16, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    table = torch.zeros((0, 3), dtype=torch.int32, device="cuda")
+    KV4.paged_kv4_append(kc, vc, row, row, slot_mapping=none)
+    KV4.paged_kv4_append(kc, vc, row, row, block_tables=table, positions=none)
+    KV4.paged_kv4_read(row, row, kc, vc, none)
+    KV4.paged_kv4_copy_slots(kc, vc, none, none, head_size=64)
+    KV4.paged_attention_kv4(row, row, kc, vc, table, none, num_kv_heads=2, scale=1.0)
+    torch.cuda.synchronize()
+    assert torch.equal(kc, before)
+
+
 def test_repeated_calls_give_the_same_bits(cuda):
     """Many short sequences with partly filled tiles and missing pages: nothing
     depends on when a fetch comes back."""

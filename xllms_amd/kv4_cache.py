@@ -24,6 +24,7 @@ from .paged_attention import NXT_ATTN_OK, PagedAttentionError, _stream_handle, k
 
 GROUP = 32  # channels that share a range
 TILE = 16   # tokens of a tile: the smallest block_size
+_MAX_STRIDE = 2**31 - 1  # the C calls take strides as int, in bytes
 
 _int32 = _uint8 = _device_of = None  # of torch, which is imported on first use
 
@@ -101,6 +102,8 @@ def _cache_args(device: int, key_cache, value_cache, kv_heads: int, head_size: i
         raise ValueError("a 4-bit cache is a uint8 tensor of 3 dimensions (kv4_cache_empty)")
     if shape != value_cache.shape or stride != value_cache.stride():
         raise ValueError("key_cache and value_cache differ in shape or strides")
+    if stride[0] > _MAX_STRIDE or stride[1] > _MAX_STRIDE:
+        raise ValueError(f"strides of {stride[0]} and {stride[1]} bytes: at most {_MAX_STRIDE}")
     if shape[1] != kv_heads:
         raise ValueError(f"the cache has {shape[1]} kv heads, not {kv_heads}")
     page = shape[2]
@@ -182,10 +185,10 @@ def paged_attention_kv4(out, query, key_cache, value_cache, block_tables, seq_le
     _pair("paged_attention_kv4", dev, out, query)
     bs, bstride, hstride = _cache_args(dev, key_cache, value_cache, num_kv_heads, head_size,
                                        block_size)
-    width = block_tables.shape[1]
+    tables = _index("block_tables", dev, block_tables, num_seqs, 2)
     status = lib.nxt_paged_attention_kv4(
         out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
-        _index("block_tables", dev, block_tables, num_seqs, 2),
-        _index("seq_lens", dev, seq_lens, num_seqs), num_seqs, num_heads, head_size, num_kv_heads,
-        float(scale), width, bs, bstride, hstride, kv_dtype_of(query), _stream_handle(stream))
+        tables, _index("seq_lens", dev, seq_lens, num_seqs), num_seqs, num_heads, head_size,
+        num_kv_heads, float(scale), block_tables.shape[1], bs, bstride, hstride,
+        kv_dtype_of(query), _stream_handle(stream))
     return _raise(lib, status, check)
